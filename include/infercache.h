@@ -54,6 +54,10 @@ enum ic_status {
 
 enum ic_dtype { IC_F32 = 0, IC_F16 = 1, IC_BF16 = 2 };
 
+/* element codes of an 8-bit page pool (the paged serving tick below; no other
+ * entry point takes such a pool) */
+enum ic_code { IC_E4M3 = 16, IC_I8 = 17 };
+
 /* ctrl words per session */
 enum ic_ctrl {
   IC_CTRL_SINK_FILL = 0,
@@ -86,6 +90,8 @@ enum ic_event_kind {
 /* device status word bits (written by kernels with bounded waits) */
 #define IC_DEVFLAG_TIMEOUT 1
 #define IC_DEVFLAG_BAD_ROW 2
+#define IC_DEVFLAG_NO_PAGES 4     /* ic_page_plan denied a session's tokens     */
+#define IC_DEVFLAG_NONFINITE 8    /* ic_page_write_q8 met an infinity or a NaN  */
 
 typedef struct ic_pool {
   void* k;                 /* [L, Hkv, pool_tokens, D] */
@@ -533,6 +539,216 @@ typedef struct ic_graph_select_args {
   int32_t* count;
 } ic_graph_select_args;
 int ic_graph_select(const ic_graph_select_args* a, void* stream);
+
+/* ======================================================================
+ * The paged serving tick: sessions of growing length over 8-bit pages.
+ *
+ * One tick is ic_page_plan (the tick's token counts become pages, slots and
+ * positions, all on the device), ic_page_write_q8 per layer (the new K / V
+ * quantised into their pages), ic_paged_attention per layer, and
+ * ic_process_logits.  The reference's paged cache is host bookkeeping around
+ * 16-bit rows (PagePool / KVAllocator, paged_cache.py:99-288) and its sampler
+ * a host loop (two_pass.py:251-279); none of these has a counterpart there.
+ *
+ * An 8-bit pool holds codes [L, H, pool_tokens, D] (one byte each, IC_E4M3 or
+ * IC_I8) and one float scale per (layer, head, page of 16 tokens) for K and
+ * for V, [L, H, pool_tokens / 16].  A stored value is code * scale.  Scales
+ * are powers of two between 2^-60 and 2^60: the smallest 2^e with
+ * max |x| <= 448 * 2^e (IC_E4M3) or 127 * 2^e (IC_I8) over the page's
+ * values, so code * scale is exact in 32 bits and scaling adds no rounding.
+ * ====================================================================== */
+
+/* ---- Block tables and slot maps from request lengths ----------------------
+ * Session s holds lens[s] tokens in the pages block_table[s, 0 ..
+ * ceil(lens[s] / 16)) and is to take counts[s] >= 0 more.  Free pages are a
+ * stack, free_pages[0 .. *free_count).  In session order, a session that needs
+ * n more pages takes the next n from the top of the stack, all or none: it is
+ * denied when counts[s] < 0, when it would outgrow its table row (width * 16
+ * tokens), when its tokens end beyond `total`, or when the pages needed up to
+ * and including it (over the sessions not denied for the first three reasons)
+ * exceed *free_count.  A denied session keeps its length and sets
+ * IC_DEVFLAG_NO_PAGES.
+ *   q_start[s]       exclusive prefix sum of counts, S + 1 entries (negative
+ *                    counts count as 0)
+ *   slots[i]         pool row (page * 16 + slot) of new token i, -1 for a
+ *                    denied session's tokens and for i >= q_start[S]
+ *   positions[i]     its position in its session, -1 likewise
+ *   lens_out[s]      lens[s] + counts[s], or lens[s] when denied
+ *   *free_count_out  what is left of the stack
+ * and the new pages are entered into block_table.  lens_out may be lens and
+ * free_count_out may be free_count (the plan is then committed at once);
+ * otherwise nothing is committed, and the same call gives the same result. */
+typedef struct ic_page_plan_args {
+  const int32_t* lens;        /* [S] */
+  const int32_t* counts;      /* [S] */
+  int32_t* block_table;       /* [S, width] */
+  const int32_t* free_pages;  /* [free_capacity] */
+  const int32_t* free_count;  /* [1] */
+  int32_t* q_start;           /* [S + 1] */
+  int32_t* slots;             /* [total] */
+  int64_t* positions;         /* [total] */
+  int32_t* lens_out;          /* [S] */
+  int32_t* free_count_out;    /* [1] */
+  int32_t* workspace;         /* [2 * S + 1] */
+  int32_t* dev_status;        /* may be NULL */
+  int32_t num_sessions;
+  int32_t width;
+  int32_t total;
+  int32_t free_capacity;
+} ic_page_plan_args;
+int ic_page_plan(const ic_page_plan_args* a, void* stream);
+
+/* ---- Give pages back --------------------------------------------------------
+ * Session s keeps its first keep[s] tokens (all of them when keep[s] >=
+ * lens[s] or keep[s] < 0; none when keep[s] = 0, the end of a request): the
+ * pages behind them go back on the stack, in session and page order from the
+ * top, so that the next plan hands them out in that order; their table entries
+ * become -1 and lens[s] = keep[s].  When a length does not fit its table row or
+ * the stack would grow past free_capacity, nothing changes and
+ * IC_DEVFLAG_BAD_ROW is set. */
+typedef struct ic_page_release_args {
+  int32_t* lens;              /* [S] */
+  const int32_t* keep;        /* [S] */
+  int32_t* block_table;       /* [S, width] */
+  int32_t* free_pages;        /* [free_capacity] */
+  int32_t* free_count;        /* [1] */
+  int32_t* dev_status;        /* may be NULL */
+  int32_t num_sessions;
+  int32_t width;
+  int32_t free_capacity;
+  int32_t _pad;
+} ic_page_release_args;
+int ic_page_release(const ic_page_release_args* a, void* stream);
+
+/* ---- Rows into and out of 8-bit pages -------------------------------------------
+ * A range names tokens and their pool rows: slots[t] (rows < 0 or past the
+ * pool are skipped by a write and read as zeros), or, with slots NULL, token
+ * start_token + t of the session whose pages are page_ids, as
+ * ic_page_rows_args.  In a write by slots the tokens of one page stand next
+ * to each other.  Element (l, h, t) of k_buf / v_buf lies at
+ * (l - layer_begin) * stride_l + h * stride_h + t * stride_t, D contiguous,
+ * every such row 16-byte aligned; buf_dtype is fp32, fp16 or bf16.
+ *
+ * A page is written in order.  Tokens that begin at its slot 0 start it anew,
+ * whatever stood there; later ones keep its scale or, when they need a
+ * larger one, raise it and round the page's other codes again to the new unit.
+ * Codes are rounded to nearest, ties to even.  Infinities are stored as the
+ * largest value, NaN as zero; both set IC_DEVFLAG_NONFINITE.
+ *
+ * A write of two ranges (or two runs of one range) to one page races; the
+ * caller keeps them disjoint, as the allocator does.  One launch handles up
+ * to IC_PAGE_BATCH_MAX ranges (`rows` is host memory, copied at the call). */
+typedef struct ic_page_q8_rows {
+  const int32_t* slots;
+  const int32_t* page_ids;
+  void* k_buf;
+  void* v_buf;
+  int64_t start_token;
+  int64_t n_tokens;
+  int64_t stride_l, stride_h, stride_t;
+  int32_t n_page_ids;
+  int32_t _pad;
+} ic_page_q8_rows;
+typedef struct ic_page_q8_args {
+  ic_pool pool;               /* dtype: IC_E4M3 or IC_I8 */
+  float* k_scale;             /* [L, H, pool_tokens / 16] */
+  float* v_scale;
+  const ic_page_q8_rows* rows;
+  int32_t* dev_status;        /* may be NULL */
+  int32_t count;
+  int32_t layer_begin, layer_end;
+  int32_t buf_dtype;
+} ic_page_q8_args;
+int ic_page_write_q8(const ic_page_q8_args* a, void* stream);
+int ic_page_read_q8(const ic_page_q8_args* a, void* stream);
+
+/* ---- Attention over 8-bit pages ----------------------------------------------------
+ * Session s has query tokens q_start[s] .. q_start[s + 1) (any number, 0
+ * among them), the last of its lens[s] held tokens: query token i of c sits at
+ * position lens[s] - c + i and attends over positions 0 .. its own (causal).
+ * Query head h reads KV head h / (Hq / Hkv):
+ *   out[t, h, :] = sum_j softmax_j(scale * q[t, h, :] . K[j]) V[j]
+ *   lse[t, h]    = natural-log log-sum-exp of the scaled scores (if lse != NULL)
+ * with K[j], V[j] = code * scale of row block_table[s, j / 16] * 16 + j % 16.
+ * A query with nothing to attend over gets zeros and -inf.  Rows of q past
+ * q_start[S] are neither read nor written.  Page ids outside the pool set
+ * IC_DEVFLAG_BAD_ROW and their tokens are left out.  Rows of a page behind the
+ * session's last token are never used, whatever they hold.
+ * Products are exact and summed in 32 bits; softmax weights enter the second
+ * product as fp16 (relative error 2^-11).
+ * k, v: one layer's codes [Hkv, pool_tokens, D] and scales [Hkv, pool_tokens /
+ * 16]; q has strides (elements), out is [num_q_tokens, Hq, D] contiguous in
+ * q's dtype (fp16 / bf16); D is 64, 128 or 256.  max_count bounds the query
+ * tokens of one session (it steers the choice of kernel only: a session with
+ * more is still computed).  workspace: ic_paged_attention_workspace(a) bytes,
+ * 16-byte aligned, not shared by calls that may overlap. */
+typedef struct ic_paged_attn_args {
+  const void* q;
+  void* out;
+  float* lse;                 /* [num_q_tokens, Hq] or NULL */
+  const void* k;
+  const void* v;
+  const float* k_scale;
+  const float* v_scale;
+  const int32_t* block_table; /* [S, table_width] */
+  const int32_t* lens;        /* [S] */
+  const int32_t* q_start;     /* [S + 1] */
+  void* workspace;
+  int64_t workspace_bytes;
+  int32_t* dev_status;        /* may be NULL */
+  int64_t pool_tokens;
+  int64_t q_stride_t, q_stride_h;
+  int32_t num_sessions, table_width, num_q_tokens, max_count;
+  int32_t num_q_heads, num_kv_heads, head_dim;
+  int32_t q_dtype;            /* IC_F16 or IC_BF16 */
+  int32_t code_dtype;         /* IC_E4M3 or IC_I8 */
+  float scale;
+} ic_paged_attn_args;
+int ic_paged_attention(const ic_paged_attn_args* a, void* stream);
+/* bytes of workspace that the call needs (0 for arguments it would refuse) */
+int64_t ic_paged_attention_workspace(const ic_paged_attn_args* a);
+
+/* ---- Penalties, biases and grammar masks on logits --------------------------------
+ * For every row r and id v, in 32 bits:
+ *   x = logits[r, v]
+ *   x = x > 0 ? x * (1 / repetition[r]) : x * repetition[r]
+ *                                     if v is among tokens[r, 0 .. token_lens[r])
+ *   x = x - (frequency[r] * n + presence[r] * (n > 0))
+ *                                     n = how often v is among tokens[r,
+ *                                     prompt_lens[r] .. token_lens[r])
+ *   x = x + bias_values[r, b]         if bias_ids[r, b] = v, b < bias_lens[r]
+ *                                     (the last such b)
+ *   x = -inf                          if bit v % 32 of mask[r, v / 32] is 0
+ *   out[r, v] = x
+ * Each part is left out when its arrays are NULL (token_lens NULL: max_tokens;
+ * prompt_lens NULL: 0; bias_lens NULL: bias_width; a penalty's array NULL: its
+ * `_all` value).  Ids outside [0, vocab) are skipped.  out may be logits when
+ * dtype is IC_F32. */
+typedef struct ic_logits_args {
+  const void* logits;         /* [rows, vocab], fp32 / fp16 / bf16 */
+  float* out;                 /* [rows, vocab] */
+  int64_t logits_stride, out_stride;      /* row strides, elements */
+  const int32_t* tokens;      /* [rows, max_tokens] */
+  const int32_t* token_lens;
+  const int32_t* prompt_lens;
+  const float* repetition;
+  const float* presence;
+  const float* frequency;
+  const int32_t* bias_ids;    /* [rows, bias_width] */
+  const float* bias_values;
+  const int32_t* bias_lens;
+  const int32_t* mask;        /* [rows, >= ceil(vocab / 32)] */
+  int64_t tokens_stride, bias_stride, mask_stride;
+  int32_t rows, vocab;
+  int32_t dtype;
+  int32_t max_tokens, bias_width;
+  float repetition_all;       /* for every row where `repetition` is NULL, with */
+  float repetition_all_inv;   /* its reciprocal (1 and 1: no penalty)            */
+  float presence_all;         /* where `presence` is NULL                        */
+  float frequency_all;        /* where `frequency` is NULL                       */
+  int32_t _pad;
+} ic_logits_args;
+int ic_process_logits(const ic_logits_args* a, void* stream);
 
 /* ---- mapped host buffers ------------------------------------------------------
  * The device address of page-locked host memory (cudaHostGetDevicePointer),

@@ -35,12 +35,14 @@ IC_CNT_TOKENS_SEEN, IC_CNT_EVICTIONS, IC_CNT_STEPS, IC_CNT_PROMOTIONS, IC_CNT_NE
 IC_SUMMARY_STATIC_MASS_MAX = 4194304  # floats of ic_summary_score_static's static scratch
 IC_COUNTER_WORDS = 8
 IC_EV_NONE, IC_EV_DROP, IC_EV_FILL, IC_EV_EVICT, IC_EV_REJECT = 0, 1, 2, 3, 4
-IC_DEVFLAG_TIMEOUT, IC_DEVFLAG_BAD_ROW = 1, 2
+IC_DEVFLAG_TIMEOUT, IC_DEVFLAG_BAD_ROW, IC_DEVFLAG_NO_PAGES, IC_DEVFLAG_NONFINITE = 1, 2, 4, 8
+IC_E4M3, IC_I8 = 16, 17  # element codes of an 8-bit page pool
 IC_DECODE_AUTO, IC_DECODE_CUDA_CORES, IC_DECODE_TENSOR_CORES, IC_DECODE_TENSOR_STREAM = 0, 1, 2, 3
 IC_DECODE_TENSOR_LEAN = 4
 IC_DECODE_TENSOR_SPLIT = 5
 
 DTYPE_CODE = {torch.float32: IC_F32, torch.float16: IC_F16, torch.bfloat16: IC_BF16}
+CODE_DTYPE = {torch.float8_e4m3fn: IC_E4M3, torch.int8: IC_I8}
 
 
 # ---- exceptions -----------------------------------------------------------------
@@ -189,6 +191,53 @@ class ic_compact_attn_args(Structure):
                 ("budget", c_int32), ("dtype", c_int32), ("scale", c_float), ("_pad", c_int32)]
 
 
+class ic_page_plan_args(Structure):
+    _fields_ = [("lens", c_void_p), ("counts", c_void_p), ("block_table", c_void_p), ("free_pages", c_void_p),
+                ("free_count", c_void_p), ("q_start", c_void_p), ("slots", c_void_p), ("positions", c_void_p),
+                ("lens_out", c_void_p), ("free_count_out", c_void_p), ("workspace", c_void_p),
+                ("dev_status", c_void_p), ("num_sessions", c_int32), ("width", c_int32), ("total", c_int32),
+                ("free_capacity", c_int32)]
+
+
+class ic_page_release_args(Structure):
+    _fields_ = [("lens", c_void_p), ("keep", c_void_p), ("block_table", c_void_p), ("free_pages", c_void_p),
+                ("free_count", c_void_p), ("dev_status", c_void_p), ("num_sessions", c_int32), ("width", c_int32),
+                ("free_capacity", c_int32), ("_pad", c_int32)]
+
+
+class ic_page_q8_rows(Structure):
+    _fields_ = [("slots", c_void_p), ("page_ids", c_void_p), ("k_buf", c_void_p), ("v_buf", c_void_p),
+                ("start_token", c_int64), ("n_tokens", c_int64), ("stride_l", c_int64), ("stride_h", c_int64),
+                ("stride_t", c_int64), ("n_page_ids", c_int32), ("_pad", c_int32)]
+
+
+class ic_page_q8_args(Structure):
+    _fields_ = [("pool", ic_pool), ("k_scale", c_void_p), ("v_scale", c_void_p), ("rows", POINTER(ic_page_q8_rows)),
+                ("dev_status", c_void_p), ("count", c_int32), ("layer_begin", c_int32), ("layer_end", c_int32),
+                ("buf_dtype", c_int32)]
+
+
+class ic_paged_attn_args(Structure):
+    _fields_ = [("q", c_void_p), ("out", c_void_p), ("lse", c_void_p), ("k", c_void_p), ("v", c_void_p),
+                ("k_scale", c_void_p), ("v_scale", c_void_p), ("block_table", c_void_p), ("lens", c_void_p),
+                ("q_start", c_void_p), ("workspace", c_void_p), ("workspace_bytes", c_int64),
+                ("dev_status", c_void_p), ("pool_tokens", c_int64), ("q_stride_t", c_int64), ("q_stride_h", c_int64),
+                ("num_sessions", c_int32), ("table_width", c_int32), ("num_q_tokens", c_int32), ("max_count", c_int32),
+                ("num_q_heads", c_int32), ("num_kv_heads", c_int32), ("head_dim", c_int32), ("q_dtype", c_int32),
+                ("code_dtype", c_int32), ("scale", c_float)]
+
+
+class ic_logits_args(Structure):
+    _fields_ = [("logits", c_void_p), ("out", c_void_p), ("logits_stride", c_int64), ("out_stride", c_int64),
+                ("tokens", c_void_p), ("token_lens", c_void_p), ("prompt_lens", c_void_p), ("repetition", c_void_p),
+                ("presence", c_void_p), ("frequency", c_void_p), ("bias_ids", c_void_p), ("bias_values", c_void_p),
+                ("bias_lens", c_void_p), ("mask", c_void_p), ("tokens_stride", c_int64), ("bias_stride", c_int64),
+                ("mask_stride", c_int64), ("rows", c_int32), ("vocab", c_int32), ("dtype", c_int32),
+                ("max_tokens", c_int32), ("bias_width", c_int32), ("repetition_all", c_float),
+                ("repetition_all_inv", c_float), ("presence_all", c_float), ("frequency_all", c_float),
+                ("_pad", c_int32)]
+
+
 # entry point name -> argument struct (None for the library-information calls)
 ENTRY_POINTS = {
     "ic_decode_layer": ic_decode_args,
@@ -211,6 +260,12 @@ ENTRY_POINTS = {
     "ic_compact_attention": ic_compact_attn_args,
     "ic_graph_push": ic_graph_push_args,
     "ic_graph_select": ic_graph_select_args,
+    "ic_page_plan": ic_page_plan_args,
+    "ic_page_release": ic_page_release_args,
+    "ic_page_write_q8": ic_page_q8_args,
+    "ic_page_read_q8": ic_page_q8_args,
+    "ic_paged_attention": ic_paged_attn_args,
+    "ic_process_logits": ic_logits_args,
 }
 # entry points over an array of argument structs: (const args*, int32 count, stream)
 BATCH_ENTRY_POINTS = {
@@ -219,7 +274,7 @@ BATCH_ENTRY_POINTS = {
 }
 IC_PAGE_BATCH_MAX = 32
 INFO_ENTRY_POINTS = ["ic_status_str", "ic_abi_version", "ic_device_check", "ic_last_error"]
-HOST_ENTRY_POINTS = ["ic_host_device_pointer", "ic_wait_probe", "ic_graph_replay"]
+HOST_ENTRY_POINTS = ["ic_host_device_pointer", "ic_wait_probe", "ic_graph_replay", "ic_paged_attention_workspace"]
 
 _LIB = None
 
@@ -255,6 +310,8 @@ def load(path: Path = LIB_PATH):
     lib.ic_wait_probe.restype = c_int
     lib.ic_graph_replay.argtypes = [POINTER(c_void_p), POINTER(c_void_p), c_int32, c_int32]
     lib.ic_graph_replay.restype = c_int
+    lib.ic_paged_attention_workspace.argtypes = [POINTER(ic_paged_attn_args)]
+    lib.ic_paged_attention_workspace.restype = c_int64
     _LIB = lib
     return lib
 

@@ -135,6 +135,7 @@ static bool same_pool(const ic_pool& x, const ic_pool& y) {
 }
 
 static int row_vecs(const ic_pool& p) {
+  if (p.dtype != IC_F32 && p.dtype != IC_F16 && p.dtype != IC_BF16) return -1;  // 8-bit pools have their own entry points
   const int esz = p.dtype == IC_F32 ? 4 : 2;
   const int bytes = p.head_dim * esz;
   if (bytes % 16 != 0 || bytes > 16 * 256) return -1;
@@ -149,7 +150,7 @@ extern "C" int ic_gather_slots(const ic_gather_args* a, void* stream) {
   if (!a) return IC_ERR_INVALID_ARG;
   if (a->n == 0 || a->layer_end == a->layer_begin) return IC_OK;
   const int vecs = row_vecs(a->pool);
-  if (vecs < 0) { set_last_error("gather_slots: row size must be a multiple of 16 bytes"); return IC_ERR_UNSUPPORTED; }
+  if (vecs < 0) { set_last_error("gather_slots: rows must be fp32 / fp16 / bf16 and a multiple of 16 bytes"); return IC_ERR_UNSUPPORTED; }
   if (a->n < 0 || !a->slots || !a->k_out || !a->v_out || !a->pool.k || !a->pool.v || !a->sess.slot_table ||
       a->session < 0 || a->session >= a->sess.num_sessions || a->layer_begin < 0 ||
       a->layer_end > a->pool.num_layers || a->layer_begin > a->layer_end) {
@@ -180,7 +181,7 @@ static int page_rows(const ic_page_rows_args* a, void* stream, bool write) {
   if (!a) return IC_ERR_INVALID_ARG;
   if (a->n_tokens == 0 || a->layer_end == a->layer_begin) return IC_OK;
   const int vecs = row_vecs(a->pool);
-  if (vecs < 0) { set_last_error("page rows: row size must be a multiple of 16 bytes"); return IC_ERR_UNSUPPORTED; }
+  if (vecs < 0) { set_last_error("page rows: rows must be fp32 / fp16 / bf16 and a multiple of 16 bytes"); return IC_ERR_UNSUPPORTED; }
   if (!page_rows_ok(a)) {
     set_last_error("page rows: bad arguments");
     return IC_ERR_INVALID_ARG;
@@ -203,7 +204,7 @@ static int page_rows_batch(const ic_page_rows_args* a, int32_t count, void* stre
     return IC_ERR_INVALID_ARG;
   }
   const int vecs = row_vecs(a[0].pool);
-  if (vecs < 0) { set_last_error("page rows: row size must be a multiple of 16 bytes"); return IC_ERR_UNSUPPORTED; }
+  if (vecs < 0) { set_last_error("page rows: rows must be fp32 / fp16 / bf16 and a multiple of 16 bytes"); return IC_ERR_UNSUPPORTED; }
   PageBatch b = {};
   b.pool = a[0].pool;
   b.layer_begin = a[0].layer_begin;

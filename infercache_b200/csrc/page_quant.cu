@@ -1,0 +1,362 @@
+// Rows into and out of 8-bit pages.
+//
+// Write: one warp per (page run, layer and head, K or V) -- a run is the
+// tokens of one call that land in one page.  The run's rows are loaded once
+// into registers, their largest magnitude gives the page scale's exponent, and
+// the codes are stored; a run that does not start its page and needs a larger
+// scale first rounds the page's other codes again.  Read: one thread per
+// 8 codes.  Both are bound by HBM: a write moves size + 1 bytes per element, a
+// read 1 + size.
+#include <stdio.h>
+
+#include "common.cuh"
+#include "launch.cuh"
+#include "q8.cuh"
+
+namespace ic {
+namespace {
+
+constexpr int WARPS = 8;  // warps per CTA (write)
+
+struct Range {
+  const int32_t* slots;
+  const int32_t* page_ids;
+  char* k_buf;
+  char* v_buf;
+  int64_t start, n, stride_l, stride_h, stride_t;
+  int64_t n_pages;
+};
+
+struct Batch {
+  uint8_t* k;
+  uint8_t* v;
+  float* k_scale;
+  float* v_scale;
+  int32_t* status;
+  int64_t pool_tokens;
+  int32_t heads, layer_begin, count;
+  int32_t window;                        // slots form of a write: tokens whose runs one warp looks after
+  int64_t first[IC_PAGE_BATCH_MAX + 1];  // work items (warps or threads) before each range
+  Range r[IC_PAGE_BATCH_MAX];
+};
+
+__device__ __forceinline__ int64_t slot_of(const Range& r, int64_t t) {
+  if (r.slots) return r.slots[t];
+  const int64_t lt = r.start + t;
+  if (lt >= r.n_pages * q8::PAGE) return -1;
+  const int32_t page = r.page_ids[lt / q8::PAGE];
+  return page < 0 ? -1 : static_cast<int64_t>(page) * q8::PAGE + lt % q8::PAGE;
+}
+
+// 4 source elements as floats from their raw bits.
+template <typename T> struct Raw4;
+template <> struct Raw4<float> {
+  using type = uint4;
+  __device__ static void floats(const uint4& u, float* o) {
+    o[0] = __uint_as_float(u.x); o[1] = __uint_as_float(u.y); o[2] = __uint_as_float(u.z); o[3] = __uint_as_float(u.w);
+  }
+};
+template <> struct Raw4<__half> {
+  using type = uint2;
+  __device__ static void floats(const uint2& u, float* o) { load4(reinterpret_cast<const __half*>(&u), o); }
+};
+template <> struct Raw4<__nv_bfloat16> {
+  using type = uint2;
+  __device__ static void floats(const uint2& u, float* o) { load4(reinterpret_cast<const __nv_bfloat16*>(&u), o); }
+};
+
+// `cnt` tokens, source rows src + t * stride (elements), into slots off ..
+// off + cnt - 1 of the page at `page` (16 rows of D codes).
+template <typename T, int D, int CODE>
+__device__ __forceinline__ void write_run(const T* src, int64_t stride, int cnt, int off, uint8_t* page, float* scale_p,
+                                          int32_t* status, int lane) {
+  constexpr int V4 = D / 4;                   // 4-element vectors per row
+  constexpr int NV = q8::PAGE * V4 / 32;      // vectors per lane for a whole page
+  using R = typename Raw4<T>::type;
+  R raw[NV];
+#pragma unroll
+  for (int j = 0; j < NV; ++j) {
+    const int it = lane + 32 * j, t = it / V4, c = it % V4;
+    raw[j] = R{};
+    if (t < cnt) raw[j] = *reinterpret_cast<const R*>(src + t * stride + 4 * c);
+  }
+  const float held = off > 0 ? *scale_p : 0.f;
+  uint32_t amax = 0;
+  bool odd = false;
+#pragma unroll
+  for (int j = 0; j < NV; ++j) {
+    float x[4];
+    Raw4<T>::floats(raw[j], x);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t b = __float_as_uint(x[i]) & 0x7fffffffu;
+      const bool finite = b < 0x7f800000u;
+      odd |= !finite;
+      amax = max(amax, finite ? b : 0u);
+    }
+  }
+  amax = __reduce_max_sync(FULL_MASK, amax);
+  if (__any_sync(FULL_MASK, odd) && lane == 0 && status) atomicOr(status, IC_DEVFLAG_NONFINITE);
+  int e = q8::exponent_for<CODE>(amax);
+  if (off > 0) {
+    const int e_old = static_cast<int>((__float_as_uint(held) >> 23) & 255u) - 127;
+    if (e > e_old) {  // round the page's other codes again to the larger unit
+      const float f = q8::two_to(max(e_old - e, -126));
+      for (int it = lane; it < q8::PAGE * V4; it += 32) {
+        const int t = it / V4;
+        if (t >= off && t < off + cnt) continue;
+        uint32_t* p = reinterpret_cast<uint32_t*>(page) + it;
+        float x[4];
+        q8::decode4<CODE>(*p, x);
+        *p = q8::encode4<CODE>(x[0] * f, x[1] * f, x[2] * f, x[3] * f);
+      }
+    } else {
+      e = q8::clamp_exp(e_old);
+    }
+  }
+  const float unit = q8::two_to(-e);
+#pragma unroll
+  for (int j = 0; j < NV; ++j) {
+    const int it = lane + 32 * j, t = it / V4;
+    if (t < cnt) {
+      float x[4];
+      Raw4<T>::floats(raw[j], x);
+      reinterpret_cast<uint32_t*>(page + off * D)[it] = q8::encode4<CODE>(x[0] * unit, x[1] * unit, x[2] * unit, x[3] * unit);
+    }
+  }
+  __syncwarp();  // every lane has read the old scale
+  if (lane == 0) *scale_p = q8::two_to(e);
+}
+
+template <typename T, int D, int CODE>
+__global__ void __launch_bounds__(WARPS * 32) write_kernel(const __grid_constant__ Batch b) {
+  grid_dependency_wait();
+  grid_launch_dependents();
+  const int lane = threadIdx.x & 31;
+  const int64_t item = static_cast<int64_t>(blockIdx.x) * WARPS + (threadIdx.x >> 5);
+  if (item >= b.first[b.count]) return;
+  int i = 0;
+  while (b.first[i + 1] <= item) ++i;
+  const Range& r = b.r[i];
+  const int64_t w = item - b.first[i];
+  const int lh = blockIdx.y, l = lh / b.heads, h = lh % b.heads;
+  const bool is_v = blockIdx.z != 0;
+  const int64_t plane = static_cast<int64_t>(b.layer_begin + l) * b.heads + h;
+  uint8_t* codes = (is_v ? b.v : b.k) + plane * b.pool_tokens * D;
+  float* scales = (is_v ? b.v_scale : b.k_scale) + plane * (b.pool_tokens / q8::PAGE);
+  const T* buf = reinterpret_cast<const T*>(is_v ? r.v_buf : r.k_buf) + l * r.stride_l + h * r.stride_h;
+
+  if (!r.slots) {  // work item w is the w-th page that the range touches
+    const int64_t page0 = (r.start / q8::PAGE + w) * q8::PAGE;
+    const int64_t t0 = max(page0 - r.start, int64_t{0}), t1 = min(page0 + q8::PAGE - r.start, r.n);
+    const int64_t slot = slot_of(r, t0);
+    if (slot < 0 || slot >= b.pool_tokens) return;
+    write_run<T, D, CODE>(buf + t0 * r.stride_t, r.stride_t, static_cast<int>(t1 - t0),
+                          static_cast<int>(slot % q8::PAGE), codes + slot / q8::PAGE * (q8::PAGE * D),
+                          scales + slot / q8::PAGE, b.status, lane);
+    return;
+  }
+  // the runs that begin among tokens w0 .. w0 + window - 1 (window <= 16):
+  // lane j holds token w0 - 1 + j's slot
+  const int64_t w0 = w * b.window, tj = w0 - 1 + lane;
+  const int32_t slot = tj >= 0 && tj < r.n ? r.slots[tj] : -1;
+  const int32_t prev = __shfl_up_sync(FULL_MASK, slot, 1);
+  const bool valid = slot >= 0 && slot < b.pool_tokens;
+  // a run goes on while the next token takes the next slot of the same page
+  const bool follows = lane > 0 && valid && prev >= 0 && slot == prev + 1 && slot % q8::PAGE != 0;
+  const uint32_t cont = __ballot_sync(FULL_MASK, follows);
+  uint32_t heads = __ballot_sync(FULL_MASK, valid && !follows && lane >= 1 && lane <= b.window);
+  while (heads) {
+    const int j = __ffs(heads) - 1;
+    heads &= heads - 1;
+    const int32_t s0 = __shfl_sync(FULL_MASK, slot, j);
+    const uint32_t rest = ~(cont >> j >> 1);  // bit k: token j + 1 + k does not go on
+    const int cnt = min(__ffs(rest), q8::PAGE - s0 % q8::PAGE);
+    write_run<T, D, CODE>(buf + (w0 - 1 + j) * r.stride_t, r.stride_t, cnt, s0 % q8::PAGE,
+                          codes + static_cast<int64_t>(s0 / q8::PAGE) * (q8::PAGE * D), scales + s0 / q8::PAGE, b.status,
+                          lane);
+    __syncwarp();
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ void store8(T* p, const float* x, float s) {
+  uint32_t u[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    T lo = DT<T>::from_f(x[2 * i] * s), hi = DT<T>::from_f(x[2 * i + 1] * s);
+    u[i] = static_cast<uint32_t>(*reinterpret_cast<uint16_t*>(&lo)) |
+           (static_cast<uint32_t>(*reinterpret_cast<uint16_t*>(&hi)) << 16);
+  }
+  *reinterpret_cast<uint4*>(p) = make_uint4(u[0], u[1], u[2], u[3]);
+}
+template <>
+__device__ __forceinline__ void store8<float>(float* p, const float* x, float s) {
+  *reinterpret_cast<float4*>(p) = make_float4(x[0] * s, x[1] * s, x[2] * s, x[3] * s);
+  *reinterpret_cast<float4*>(p + 4) = make_float4(x[4] * s, x[5] * s, x[6] * s, x[7] * s);
+}
+
+template <typename T, int CODE>
+__global__ void __launch_bounds__(256) read_kernel(const __grid_constant__ Batch b, int D) {
+  grid_dependency_wait();
+  grid_launch_dependents();
+  const int64_t item = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x;
+  if (item >= b.first[b.count]) return;
+  int i = 0;
+  while (b.first[i + 1] <= item) ++i;
+  const Range& r = b.r[i];
+  const int v8 = D / 8;
+  const int64_t t = (item - b.first[i]) / v8;
+  const int c = static_cast<int>((item - b.first[i]) % v8);
+  const int lh = blockIdx.y, l = lh / b.heads, h = lh % b.heads;
+  const bool is_v = blockIdx.z != 0;
+  const int64_t plane = static_cast<int64_t>(b.layer_begin + l) * b.heads + h;
+  T* out = reinterpret_cast<T*>(is_v ? r.v_buf : r.k_buf) + l * r.stride_l + h * r.stride_h + t * r.stride_t + 8 * c;
+  const int64_t slot = slot_of(r, t);
+  float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, s = 0.f;
+  if (slot >= 0 && slot < b.pool_tokens) {
+    const uint8_t* codes = (is_v ? b.v : b.k) + (plane * b.pool_tokens + slot) * D;
+    const uint2 u = reinterpret_cast<const uint2*>(codes)[c];
+    s = (is_v ? b.v_scale : b.k_scale)[plane * (b.pool_tokens / q8::PAGE) + slot / q8::PAGE];
+    q8::decode4<CODE>(u.x, x);
+    q8::decode4<CODE>(u.y, x + 4);
+  }
+  store8<T>(out, x, s);
+}
+
+bool q8_args_ok(const ic_page_q8_args* a, const char* name) {
+  char msg[160];
+  const auto fail = [&](const char* why) {
+    snprintf(msg, sizeof(msg), "%s: %s", name, why);
+    set_last_error(msg);
+    return false;
+  };
+  if (!a || !a->rows || !a->pool.k || !a->pool.v || !a->k_scale || !a->v_scale) return fail("null argument");
+  if (a->pool.dtype != IC_E4M3 && a->pool.dtype != IC_I8) return fail("the pool must hold 8-bit codes");
+  if (a->count < 1 || a->count > IC_PAGE_BATCH_MAX) return fail("1 <= count <= IC_PAGE_BATCH_MAX ranges");
+  if (a->pool.num_layers < 1 || a->pool.num_kv_heads < 1 || a->pool.pool_tokens < q8::PAGE ||
+      a->pool.pool_tokens % q8::PAGE || a->pool.pool_tokens > 0x7fffffff || a->layer_begin < 0 ||
+      a->layer_end > a->pool.num_layers || a->layer_begin > a->layer_end)
+    return fail("bad pool or layer range");
+  if (static_cast<int64_t>(a->layer_end - a->layer_begin) * a->pool.num_kv_heads > 65535)
+    return fail("more than 65535 layers times heads");
+  if (a->buf_dtype != IC_F32 && a->buf_dtype != IC_F16 && a->buf_dtype != IC_BF16) return fail("bad buffer dtype");
+  if ((reinterpret_cast<uintptr_t>(a->pool.k) & 15) || (reinterpret_cast<uintptr_t>(a->pool.v) & 15))
+    return fail("the pool must be 16-byte aligned");
+  const int esz = a->buf_dtype == IC_F32 ? 4 : 2;
+  for (int i = 0; i < a->count; ++i) {
+    const ic_page_q8_rows& r = a->rows[i];
+    if (r.n_tokens < 0 || r.n_tokens > 0x7fffffff) return fail("bad token count");
+    if (r.n_tokens == 0) continue;
+    if (!r.k_buf || !r.v_buf || (!r.slots && !r.page_ids)) return fail("null buffer, slots or pages");
+    if (!r.slots && (r.start_token < 0 || r.start_token + r.n_tokens > static_cast<int64_t>(r.n_page_ids) * q8::PAGE))
+      return fail("tokens past the page list");
+    if ((r.stride_l * esz) % 16 || (r.stride_h * esz) % 16 || (r.stride_t * esz) % 16 ||
+        (reinterpret_cast<uintptr_t>(r.k_buf) & 15) || (reinterpret_cast<uintptr_t>(r.v_buf) & 15))
+      return fail("buffer rows must be 16-byte aligned");
+  }
+  return true;
+}
+
+int q8_dim_error(const char* name) {
+  char msg[96];
+  snprintf(msg, sizeof(msg), "%s: head_dim must be 64, 128 or 256", name);
+  set_last_error(msg);
+  return IC_ERR_UNSUPPORTED;
+}
+
+void fill_batch(const ic_page_q8_args* a, Batch& b) {
+  b.k = static_cast<uint8_t*>(a->pool.k);
+  b.v = static_cast<uint8_t*>(a->pool.v);
+  b.k_scale = a->k_scale;
+  b.v_scale = a->v_scale;
+  b.status = a->dev_status;
+  b.pool_tokens = a->pool.pool_tokens;
+  b.heads = a->pool.num_kv_heads;
+  b.layer_begin = a->layer_begin;
+  b.count = a->count;
+  for (int i = 0; i < a->count; ++i) {
+    const ic_page_q8_rows& r = a->rows[i];
+    b.r[i] = Range{r.slots, r.page_ids, static_cast<char*>(r.k_buf), static_cast<char*>(r.v_buf), r.start_token,
+                   r.n_tokens, r.stride_l, r.stride_h, r.stride_t, r.n_page_ids};
+  }
+}
+
+template <typename T, int D>
+const void* write_fn(int code) {
+  return code == IC_E4M3 ? reinterpret_cast<const void*>(write_kernel<T, D, IC_E4M3>)
+                         : reinterpret_cast<const void*>(write_kernel<T, D, IC_I8>);
+}
+template <typename T>
+const void* write_fn_d(int d, int code) {
+  return d == 64 ? write_fn<T, 64>(code) : d == 128 ? write_fn<T, 128>(code) : write_fn<T, 256>(code);
+}
+template <typename T>
+const void* read_fn(int code) {
+  return code == IC_E4M3 ? reinterpret_cast<const void*>(read_kernel<T, IC_E4M3>)
+                         : reinterpret_cast<const void*>(read_kernel<T, IC_I8>);
+}
+
+}  // namespace
+}  // namespace ic
+
+extern "C" int ic_page_write_q8(const ic_page_q8_args* a, void* stream) {
+  using namespace ic;
+  if (!q8_args_ok(a, "page_write_q8")) return IC_ERR_INVALID_ARG;
+  const int D = a->pool.head_dim;
+  if (D != 64 && D != 128 && D != 256) return q8_dim_error("page_write_q8");
+  const int planes = (a->layer_end - a->layer_begin) * a->pool.num_kv_heads;
+  if (planes == 0) return IC_OK;
+  Batch b = {};
+  fill_batch(a, b);
+  // Slots form: a warp looks after one token's run when that still leaves few
+  // warps (a decode tick: every run is one token and all run side by side),
+  // else after the runs that begin among 16 tokens, so that a prompt's warps
+  // have a page each instead of fifteen in sixteen finding nothing to do.
+  int64_t tokens = 0;
+  for (int i = 0; i < a->count; ++i) tokens += a->rows[i].n_tokens;
+  b.window = tokens * planes <= 16384 ? 1 : 16;
+  for (int i = 0; i < a->count; ++i) {
+    const ic_page_q8_rows& r = a->rows[i];
+    const int64_t items = r.n_tokens == 0 ? 0
+                          : r.slots      ? (r.n_tokens + b.window - 1) / b.window
+                                         : (r.start_token + r.n_tokens - 1) / q8::PAGE - r.start_token / q8::PAGE + 1;
+    b.first[i + 1] = b.first[i] + items;
+  }
+  const int64_t blocks = (b.first[b.count] + WARPS - 1) / WARPS;
+  if (blocks == 0) return IC_OK;
+  if (blocks > 0x7fffffff) {
+    set_last_error("page_write_q8: too many tokens for one launch");
+    return IC_ERR_UNSUPPORTED;
+  }
+  const void* fn = a->buf_dtype == IC_F32   ? write_fn_d<float>(D, a->pool.dtype)
+                   : a->buf_dtype == IC_F16 ? write_fn_d<__half>(D, a->pool.dtype)
+                                            : write_fn_d<__nv_bfloat16>(D, a->pool.dtype);
+  void* p[] = {&b};
+  return launch_pdl(fn, dim3(static_cast<unsigned>(blocks), planes, 2), dim3(WARPS * 32), 0,
+                    static_cast<cudaStream_t>(stream), p, "page_write_q8");
+}
+
+extern "C" int ic_page_read_q8(const ic_page_q8_args* a, void* stream) {
+  using namespace ic;
+  if (!q8_args_ok(a, "page_read_q8")) return IC_ERR_INVALID_ARG;
+  int D = a->pool.head_dim;
+  if (D != 64 && D != 128 && D != 256) return q8_dim_error("page_read_q8");
+  const int planes = (a->layer_end - a->layer_begin) * a->pool.num_kv_heads;
+  if (planes == 0) return IC_OK;
+  Batch b = {};
+  fill_batch(a, b);
+  for (int i = 0; i < a->count; ++i) b.first[i + 1] = b.first[i] + a->rows[i].n_tokens * (D / 8);
+  const int64_t blocks = (b.first[b.count] + 255) / 256;
+  if (blocks == 0) return IC_OK;
+  if (blocks > 0x7fffffff) {
+    set_last_error("page_read_q8: too many tokens for one launch");
+    return IC_ERR_UNSUPPORTED;
+  }
+  const void* fn = a->buf_dtype == IC_F32   ? read_fn<float>(a->pool.dtype)
+                   : a->buf_dtype == IC_F16 ? read_fn<__half>(a->pool.dtype)
+                                            : read_fn<__nv_bfloat16>(a->pool.dtype);
+  void* p[] = {&b, &D};
+  return launch_pdl(fn, dim3(static_cast<unsigned>(blocks), planes, 2), dim3(256), 0, static_cast<cudaStream_t>(stream),
+                    p, "page_read_q8");
+}

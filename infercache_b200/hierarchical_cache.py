@@ -101,6 +101,7 @@ def _check_cfg(cfg: CacheConfig) -> None:
         raise ValueError("tier sizes must be >= 0")
     if not (0.0 < cfg.decay <= 1.0):
         raise ValueError(f"decay must be in (0, 1], got {cfg.decay}")
+    _lib.dtype_code(cfg.dtype)  # an 8-bit pool's pages are written in order: no budgeted session lives in one
 
 
 class SessionBatch:

@@ -10,7 +10,9 @@ so the budgeted ``HierarchicalKVCache`` sessions and the append-only
 
 What changes is where the bytes move: token writes and session gathers are
 single kernel launches over all layers and tokens (``ic_page_write`` /
-``ic_page_gather``) instead of per-token, per-layer Python indexing.  The
+``ic_page_gather``) instead of per-token, per-layer Python indexing.  A pool of
+dtype float8_e4m3fn or int8 stores codes with a scale per page, layer and head
+(``ic_page_write_q8`` / ``ic_page_read_q8``) behind the same methods.  The
 allocator stays on the host, as in the reference (a free list and an LRU map
 under a lock, paged_cache.py:205-288).
 """
@@ -27,6 +29,7 @@ import numpy as np
 import torch
 
 from . import _lib
+from .paged_ops import HEAD_DIMS, rows16
 
 __all__ = ["PAGE_SIZE", "PagePool", "KVAllocator", "MultiSessionCache", "PagedSessionView",
            "PagedCacheConfig"]
@@ -44,12 +47,22 @@ class PagedCacheConfig:
     dtype: torch.dtype = torch.float16
     device: str = "cuda"
     max_pages_per_session: int = 64
+    # dtype float8_e4m3fn or int8 makes an 8-bit pool: codes with one power-of-two
+    # scale per page, layer and head; its rows are read back as value_dtype
+    value_dtype: torch.dtype = torch.float16
 
     @property
     def total_tokens(self) -> int:
         return self.n_pages * PAGE_SIZE
 
+    @property
+    def quantised(self) -> bool:
+        return self.dtype in _lib.CODE_DTYPE
+
     def gpu_memory_mb(self) -> float:
+        if self.quantised:
+            planes = 2 * self.n_layers * self.n_heads
+            return planes * (self.total_tokens * self.head_dim + self.n_pages * 4) / (1024 ** 2)
         bytes_per_elem = 2 if self.dtype == torch.float16 else 4
         total = 2 * self.n_layers * self.n_heads * self.total_tokens * self.head_dim
         return total * bytes_per_elem / (1024 ** 2)
@@ -62,10 +75,26 @@ class PagePool:
         self.cfg = cfg
         dev = torch.device(cfg.device)
         _lib.require_device(dev)
-        _lib.dtype_code(cfg.dtype)
         total = cfg.n_pages * PAGE_SIZE
+        self.quantised = cfg.quantised
+        if self.quantised:
+            self._init_quantised(cfg, dev, total)
+            return
+        _lib.dtype_code(cfg.dtype)
         self.K = torch.zeros(cfg.n_layers, cfg.n_heads, total, cfg.head_dim, dtype=cfg.dtype, device=dev)
         self.V = torch.zeros(cfg.n_layers, cfg.n_heads, total, cfg.head_dim, dtype=cfg.dtype, device=dev)
+        self._c_pool = self.c_pool()
+
+    def _init_quantised(self, cfg: PagedCacheConfig, dev: torch.device, total: int) -> None:
+        _lib.dtype_code(cfg.value_dtype)
+        if cfg.head_dim not in HEAD_DIMS:
+            raise ValueError(f"an 8-bit pool needs head_dim in {HEAD_DIMS}, got {cfg.head_dim}")
+        shape = (cfg.n_layers, cfg.n_heads, total, cfg.head_dim)
+        self.K, self.V = (torch.zeros(shape, dtype=torch.uint8, device=dev).view(cfg.dtype) for _ in range(2))
+        self.k_scale, self.v_scale = (torch.zeros((cfg.n_layers, cfg.n_heads, cfg.n_pages), dtype=torch.float32,
+                                                  device=dev) for _ in range(2))
+        # IC_DEVFLAG_* bits of the writes (an infinity or a NaN was stored as something finite)
+        self.dev_status = torch.zeros(1, dtype=torch.int32, device=dev)
         self._c_pool = self.c_pool()
 
     @classmethod
@@ -89,7 +118,45 @@ class PagePool:
         c = self.cfg
         return _lib.ic_pool(k=self.K.data_ptr(), v=self.V.data_ptr(), pool_tokens=c.n_pages * PAGE_SIZE,
                             num_layers=c.n_layers, num_kv_heads=c.n_heads, head_dim=c.head_dim,
-                            dtype=_lib.dtype_code(c.dtype))
+                            dtype=_lib.CODE_DTYPE[c.dtype] if c.quantised else _lib.dtype_code(c.dtype))
+
+    @property
+    def value_dtype(self) -> torch.dtype:
+        """What rows are read back as: the pool's dtype, value_dtype for an 8-bit pool."""
+        return self.cfg.value_dtype if self.quantised else self.cfg.dtype
+
+    # -- 8-bit rows: a page is written in order (its slot 0 starts it anew) ---------------
+    def _q8_rows(self, page_ids: torch.Tensor, n_page_ids: int, start: int, k: torch.Tensor,
+                 v: torch.Tensor) -> _lib.ic_page_q8_rows:
+        return _lib.ic_page_q8_rows(page_ids=page_ids.data_ptr(), n_page_ids=n_page_ids, k_buf=k.data_ptr(),
+                                    v_buf=v.data_ptr(), start_token=start, n_tokens=k.shape[2], stride_l=k.stride(0),
+                                    stride_h=k.stride(1), stride_t=k.stride(2))
+
+    def _q8_call(self, name: str, rows: List[_lib.ic_page_q8_rows], layer_begin: int, layer_end: int,
+                 dtype: torch.dtype) -> None:
+        with torch.cuda.device(self.device):
+            for i in range(0, len(rows), _lib.IC_PAGE_BATCH_MAX):
+                part = rows[i:i + _lib.IC_PAGE_BATCH_MAX]
+                arr = (_lib.ic_page_q8_rows * len(part))(*part)
+                _lib.call(name, _lib.ic_page_q8_args(
+                    pool=self._c_pool, k_scale=self.k_scale.data_ptr(), v_scale=self.v_scale.data_ptr(), rows=arr,
+                    dev_status=self.dev_status.data_ptr(), count=len(part), layer_begin=layer_begin,
+                    layer_end=layer_end, buf_dtype=_lib.dtype_code(dtype)))
+
+    def _q8_source(self, k: torch.Tensor, v: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
+        """k, v on the device, in one floating dtype (k's), rows aligned for the kernel."""
+        k = k.to(self.device)
+        v = v.to(self.device, k.dtype)
+        if k.stride() != v.stride() or not rows16(k) or not rows16(v):
+            k, v = (t.clone(memory_format=torch.contiguous_format) for t in (k, v))
+        return k, v
+
+    def check_device_status(self) -> None:
+        """Raise if a write into an 8-bit pool met an infinity or a NaN since the
+        last check (synchronises)."""
+        if self.quantised and int(self.dev_status.item()):
+            self.dev_status.zero_()
+            raise _lib.InvalidArgument(_lib.IC_ERR_INVALID_ARG, "an infinity or a NaN was written into an 8-bit pool")
 
     def _abs(self, page_id: int, slot: int) -> int:
         return page_id * PAGE_SIZE + slot
@@ -104,6 +171,13 @@ class PagePool:
                    layer_begin: int = 0) -> None:
         """Write k, v [L', H, T, D] as tokens start_token .. start_token+T-1 of
         the session whose pages are `page_ids`, layers layer_begin .. +L'."""
+        if self.quantised:
+            if k.shape[0] and k.shape[2]:
+                k, v = self._q8_source(k, v)
+                pid = self._page_ids(page_ids)
+                self._q8_call("ic_page_write_q8", [self._q8_rows(pid, len(page_ids), start_token, k, v)], layer_begin,
+                              layer_begin + k.shape[0], k.dtype)
+            return
         k = k.to(self.device, self.cfg.dtype)
         v = v.to(self.device, self.cfg.dtype)
         # strided sources go to the kernel as they are (rows must be contiguous)
@@ -127,11 +201,14 @@ class PagePool:
                     layer_end: int) -> Tuple[torch.Tensor, torch.Tensor]:
         c = self.cfg
         nl = layer_end - layer_begin
-        K = torch.empty(nl, c.n_heads, n_tokens, c.head_dim, dtype=c.dtype, device=self.device)
+        K = torch.empty(nl, c.n_heads, n_tokens, c.head_dim, dtype=self.value_dtype, device=self.device)
         V = torch.empty_like(K)
         if n_tokens == 0 or nl == 0:
             return K, V
         pid = self._page_ids(page_ids)
+        if self.quantised:
+            self._q8_call("ic_page_read_q8", [self._q8_rows(pid, len(page_ids), 0, K, V)], layer_begin, layer_end, K.dtype)
+            return K, V
         a = _lib.ic_page_rows_args(pool=self._c_pool, page_ids=pid.data_ptr(), n_page_ids=len(page_ids),
                                    layer_begin=layer_begin, layer_end=layer_end, start_token=0,
                                    n_tokens=n_tokens, k_buf=K.data_ptr(), v_buf=V.data_ptr(),
@@ -156,6 +233,19 @@ class PagePool:
         """write_rows for several page lists, all layers from 0: items are
         (page_ids, start_token, k, v) with k, v [L, H, T, D]; one launch per
         IC_PAGE_BATCH_MAX items.  The page lists must not share pool rows."""
+        if self.quantised:
+            by_dtype: Dict[torch.dtype, list] = {}
+            keep = []
+            for page_ids, start, k, v in items:
+                if k.shape[2] == 0:
+                    continue
+                k, v = self._q8_source(k, v)
+                pid = self._page_ids(page_ids)
+                keep.append((pid, k, v))
+                by_dtype.setdefault(k.dtype, []).append(self._q8_rows(pid, len(page_ids), start, k, v))
+            for dtype, rows in by_dtype.items():
+                self._q8_call("ic_page_write_q8", rows, 0, self.cfg.n_layers, dtype)
+            return
         descs, keep = [], []
         for page_ids, start, k, v in items:
             if k.shape[2] == 0:
@@ -175,29 +265,39 @@ class PagePool:
         `out`, if given, holds a (K, V) pair per item to gather into: tensors of
         the pool's dtype and device, shape [n_layers, n_heads, n_tokens,
         head_dim], rows contiguous and 16-byte aligned."""
-        c = self.cfg
-        outs, descs = [], []
+        c, dtype = self.cfg, self.value_dtype
+        outs, descs, keep = [], [], []
         for i, (page_ids, n) in enumerate(items):
             if out is None:
-                K = torch.empty(c.n_layers, c.n_heads, n, c.head_dim, dtype=c.dtype, device=self.device)
+                K = torch.empty(c.n_layers, c.n_heads, n, c.head_dim, dtype=dtype, device=self.device)
                 V = torch.empty_like(K)
             else:
                 K, V = out[i]
                 shape = (c.n_layers, c.n_heads, n, c.head_dim)
                 for x in (K, V):
-                    if tuple(x.shape) != shape or x.dtype != c.dtype or x.device != self.device or x.stride(-1) != 1:
-                        raise ValueError(f"gather_rows_many: out[{i}] must be {shape} {c.dtype} on {self.device} "
+                    if tuple(x.shape) != shape or x.dtype != dtype or x.device != self.device or x.stride(-1) != 1:
+                        raise ValueError(f"gather_rows_many: out[{i}] must be {shape} {dtype} on {self.device} "
                                          "with contiguous rows")
             outs.append((K, V))
             if n > 0:
-                descs.append(self._rows_args(self._page_ids(page_ids), len(page_ids), 0, K, V, 0))
-        self._run_batches("ic_page_gather_batch", descs)
+                pid = self._page_ids(page_ids)
+                keep.append(pid)
+                if self.quantised:
+                    if K.stride() != V.stride():
+                        raise ValueError(f"gather_rows_many: out[{i}]'s K and V must have the same strides")
+                    descs.append(self._q8_rows(pid, len(page_ids), 0, K, V))
+                else:
+                    descs.append(self._rows_args(pid, len(page_ids), 0, K, V, 0))
+        if self.quantised:
+            self._q8_call("ic_page_read_q8", descs, 0, c.n_layers, dtype)
+        else:
+            self._run_batches("ic_page_gather_batch", descs)
         return outs
 
     def gather_session(self, layer: int, page_ids: List[int], n_tokens: int) -> Tuple[torch.Tensor, torch.Tensor]:
         """K, V [n_heads, n_tokens, head_dim] (paged_cache.py:172-200)."""
         if len(page_ids) == 0:
-            empty = torch.zeros(self.cfg.n_heads, 0, self.cfg.head_dim, dtype=self.cfg.dtype, device=self.device)
+            empty = torch.zeros(self.cfg.n_heads, 0, self.cfg.head_dim, dtype=self.value_dtype, device=self.device)
             return empty, empty
         n_tokens = min(n_tokens, len(page_ids) * PAGE_SIZE)
         K, V = self.gather_rows(page_ids, n_tokens, layer, layer + 1)

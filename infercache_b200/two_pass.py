@@ -29,6 +29,7 @@ import torch
 from . import hf_attention
 from .cache_safety import normalise_kv
 from .hierarchical_cache import CacheConfig, HierarchicalKVCache
+from .logits import process_logits
 
 
 @dataclass
@@ -105,9 +106,14 @@ class TwoPassEngine:
         cfg = self.cfg
         logits = logits.float().clone()
         if cfg.repetition_penalty != 1.0 and generated:
-            for tok in set(generated):
-                logits[tok] = logits[tok] / cfg.repetition_penalty if logits[tok] > 0 \
-                    else logits[tok] * cfg.repetition_penalty
+            if logits.is_cuda:
+                row = logits.view(1, -1)
+                said = torch.tensor([generated], dtype=torch.int32).to(logits.device, non_blocking=True)
+                process_logits(row, tokens=said, repetition=cfg.repetition_penalty, out=row)
+            else:  # logits that the caller keeps on the host
+                for tok in set(generated):
+                    logits[tok] = logits[tok] / cfg.repetition_penalty if logits[tok] > 0 \
+                        else logits[tok] * cfg.repetition_penalty
         if cfg.temperature < 1e-4:
             return int(logits.argmax(-1).item())
         logits /= cfg.temperature
