@@ -8,6 +8,7 @@ calls that need it raise.
 from __future__ import annotations
 
 import ctypes
+import importlib.util
 import os
 from ctypes import POINTER, Structure, c_char_p, c_float, c_int, c_int32, c_int64, c_void_p
 from pathlib import Path
@@ -15,6 +16,7 @@ from pathlib import Path
 import torch
 
 LIB_PATH = Path(__file__).resolve().parent / "lib" / "libinfercache_b200.so"
+BINDING_PATH = LIB_PATH.with_name("_binding.so")
 
 # ---- enums (infercache.h) ----------------------------------------------------
 IC_OK = 0
@@ -314,6 +316,24 @@ def load(path: Path = LIB_PATH):
     lib.ic_paged_attention_workspace.restype = c_int64
     _LIB = lib
     return lib
+
+
+_BINDING = None
+
+
+def binding():
+    """The compiled binding of the paged serving tick (csrc/binding.cpp), loaded once."""
+    global _BINDING
+    if _BINDING is None:
+        load()
+        if not BINDING_PATH.exists():
+            raise ImportError(f"{BINDING_PATH} is missing: run `python -m infercache_b200.build`")
+        spec = importlib.util.spec_from_file_location("infercache_b200._binding", BINDING_PATH)
+        module = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(module)
+        module.setup(require_device, raise_for)
+        _BINDING = module
+    return _BINDING
 
 
 def raise_for(status: int, what: str = "") -> None:

@@ -1,11 +1,13 @@
-"""Build the sm_100a C-ABI library in-tree.
+"""Build the sm_100a C-ABI library and its Python binding in-tree.
 
     python -m infercache_b200.build [--force] [--verbose]
 
 Compiles every ``csrc/*.cu`` with nvcc for ``sm_100a`` (cross-compiles on a
 machine without a GPU) and links ``lib/libinfercache_b200.so`` with the CUDA
 runtime linked statically, so the library does not depend on which
-libcudart the host process loaded first.
+libcudart the host process loaded first.  Then compiles ``csrc/binding.cpp``
+(the paged serving tick's calls on torch tensors) with g++ against the torch
+that runs this, as ``lib/_binding.so``.
 """
 from __future__ import annotations
 
@@ -23,6 +25,7 @@ CSRC = PKG / "csrc"
 OBJ = PKG / "_build"
 LIBDIR = PKG / "lib"
 LIB = LIBDIR / "libinfercache_b200.so"
+BINDING = LIBDIR / "_binding.so"
 HEADERS = [ROOT / "include" / "infercache.h"] + sorted(CSRC.glob("*.cuh"))
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
@@ -73,7 +76,29 @@ def build(force: bool = False, verbose: bool = False) -> Path:
         if r.returncode != 0:
             sys.stderr.write(r.stdout + r.stderr)
             raise RuntimeError("link failed")
+    build_binding(force)
     return LIB
+
+
+def build_binding(force: bool = False) -> Path:
+    src = CSRC / "binding.cpp"
+    if not force and not _stale(BINDING, [src, ROOT / "include" / "infercache.h"]):
+        return BINDING
+    import sysconfig
+
+    import torch
+    from torch.utils.cpp_extension import include_paths, library_paths
+    inc = include_paths() + [sysconfig.get_paths()["include"], str(Path(nvcc()).resolve().parents[1] / "include")]
+    cmd = [shutil.which("g++") or "g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}", *(f"-I{d}" for d in inc), str(src),
+           "-o", str(BINDING), f"-L{LIBDIR}", "-linfercache_b200", "-Wl,-rpath,$ORIGIN",
+           *(f"-L{d}" for d in library_paths()), *(f"-Wl,-rpath,{d}" for d in library_paths()),
+           "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_cuda", "-ltorch_python"]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        sys.stderr.write(r.stdout + r.stderr)
+        raise RuntimeError("g++ failed on binding.cpp")
+    return BINDING
 
 
 def main():
