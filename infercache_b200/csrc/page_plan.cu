@@ -17,107 +17,131 @@
 namespace ic {
 namespace {
 
-constexpr int PT = 1024;            // threads of the scanning CTA
-constexpr int TPT = 8;              // consecutive tokens per thread
+constexpr int PT = 1024;            // most threads of the scanning CTA
+constexpr int TPT = 8;              // tokens per thread
+constexpr int WT = 32 * TPT;        // consecutive tokens per warp
 // Tokens that the scanning CTA finishes itself: one pass of its threads.
 constexpr int FUSED_TOKENS = PT * TPT;
 
 // Inclusive block scan of one int64 per thread; `total` gets the block's sum.
 __device__ __forceinline__ int64_t block_scan(int64_t v, int64_t* warp_sums, int64_t& total) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
     const int64_t u = __shfl_up_sync(FULL_MASK, v, o);
     if (lane >= o) v += u;
   }
+  if (warps == 1) {
+    total = __shfl_sync(FULL_MASK, v, 31);
+    return v;
+  }
   if (lane == 31) warp_sums[warp] = v;
   __syncthreads();
-  if (warp == 0) {
-    int64_t w = lane < static_cast<int>(blockDim.x >> 5) ? warp_sums[lane] : 0;
+  int64_t w = lane < warps ? warp_sums[lane] : 0;  // every warp scans the warps' sums for itself
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int64_t u = __shfl_up_sync(FULL_MASK, w, o);
-      if (lane >= o) w += u;
-    }
-    warp_sums[lane] = w;
+  for (int o = 1; o < 32; o <<= 1) {
+    const int64_t u = __shfl_up_sync(FULL_MASK, w, o);
+    if (lane >= o) w += u;
   }
-  __syncthreads();
-  total = warp_sums[31];
-  const int64_t r = v + (warp > 0 ? warp_sums[warp - 1] : 0);
+  total = __shfl_sync(FULL_MASK, w, 31);
+  const int64_t before = __shfl_sync(FULL_MASK, w, warp > 0 ? warp - 1 : 0);
   __syncthreads();  // warp_sums may be written again
-  return r;
+  return v + (warp > 0 ? before : 0);
 }
 
 __device__ __forceinline__ int32_t pages_of(int64_t tokens) {
   return static_cast<int32_t>((tokens + q8::PAGE - 1) / q8::PAGE);
 }
 
-// One thread's TPT tokens.  work[2s] is session s's length before the call (-1
-// when it was denied), work[2s + 1] its first new page's rank, work[2S] the
-// stack's height before the call.
-__device__ __forceinline__ void plan_tokens(const ic_page_plan_args& a, const int32_t* q_start, const int32_t* work,
-                                            int64_t i0) {
-  const int S = a.num_sessions;
-  const int64_t n = a.total;
-  if (i0 >= n) return;
-  // the last session with q_start[s] <= i0 (empty sessions before it are skipped)
-  int lo = 0, hi = S;
+// A warp's tokens [i0, i1), i0 a multiple of WT.  len[s] is session s's length
+// before the call (-1 when it was denied), rank[s] its first new page's rank,
+// `top` the stack's height before the call.
+__device__ __forceinline__ void plan_tokens(const ic_page_plan_args& a, const int32_t* q_start, const int32_t* len,
+                                            const int32_t* rank, int stride, int32_t top, int64_t i0, int64_t i1) {
+  const int S = a.num_sessions, lane = threadIdx.x & 31;
+  if (i0 >= i1) return;
+  int lo = 0, hi = S;  // the last session with q_start[s] <= i0
   while (hi - lo > 1) {
     const int mid = (lo + hi) >> 1;
     if (q_start[mid] <= i0) lo = mid; else hi = mid;
   }
   int s = lo;
-  const int32_t top = work[2 * S];
-  int32_t slot[TPT];
-  int64_t pos[TPT];
-  int32_t begin = q_start[s], end = q_start[s + 1], held_len = work[2 * s], rank = work[2 * s + 1];
-  int32_t page_at = -1, page = -1;  // the page id last looked up, and its index in the session
-#pragma unroll
-  for (int j = 0; j < TPT; ++j) {
-    const int64_t i = i0 + j;
-    while (i >= end && s + 1 < S) {
+  int64_t begin = q_start[s], end = q_start[s + 1];
+  const bool vec = ((reinterpret_cast<uintptr_t>(a.slots) & 7) | (reinterpret_cast<uintptr_t>(a.positions) & 15)) == 0;
+  const auto held_of = [&](int x) { return len[static_cast<int64_t>(x) * stride]; };
+  const auto rank_of = [&](int x) { return rank[static_cast<int64_t>(x) * stride]; };
+#pragma unroll 1
+  for (; i0 < i1; i0 += WT) {
+    while (i0 >= end && s + 1 < S) {
       ++s;
       begin = end;
       end = q_start[s + 1];
-      held_len = work[2 * s];
-      rank = work[2 * s + 1];
-      page_at = -1;
     }
-    slot[j] = -1;
-    pos[j] = -1;
-    if (i < n && i < end && held_len >= 0) {
-      const int64_t p = held_len + (i - begin);
-      const int32_t idx = static_cast<int32_t>(p / q8::PAGE), held = pages_of(held_len);
+    const int32_t had = held_of(s);
+    if (vec && had >= 0 && i0 >= begin && i0 + WT <= end && i0 + WT <= i1) {
+      // all of them are one session's: everything but the token's number is uniform
+      const uint32_t held = static_cast<uint32_t>(pages_of(had));
       int32_t* row = a.block_table + static_cast<int64_t>(s) * a.width;
-      if (idx != page_at) {
-        page = idx < held ? row[idx] : a.free_pages[top - 1 - (rank + idx - held)];
-        page_at = idx;
+      const int32_t* fresh = a.free_pages + (top - 1 - rank_of(s)) + static_cast<int64_t>(held);  // page idx: fresh[-idx]
+      const uint32_t p0 = static_cast<uint32_t>(had) + static_cast<uint32_t>(i0 - begin) + 2 * lane;
+      int32_t page[TPT];
+#pragma unroll
+      for (int j = 0; j < TPT; ++j) {
+        const uint32_t p = p0 + 64 * (j >> 1) + (j & 1), idx = p / q8::PAGE;
+        if ((j & 1) && p % q8::PAGE != 0)
+          page[j] = page[j - 1];
+        else
+          page[j] = idx < held ? row[idx] : fresh[-static_cast<int64_t>(idx)];
       }
-      if (idx >= held && p % q8::PAGE == 0) row[idx] = page;  // a new page's first token enters it
-      slot[j] = page < 0 ? -1 : page * q8::PAGE + static_cast<int32_t>(p % q8::PAGE);
-      pos[j] = p;
+#pragma unroll
+      for (int j = 0; j < TPT; j += 2) {
+        int32_t slot[2];
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          const uint32_t p = p0 + 64 * (j >> 1) + k;
+          if (p % q8::PAGE == 0 && p / q8::PAGE >= held) row[p / q8::PAGE] = page[j + k];
+          slot[k] = page[j + k] < 0 ? -1 : page[j + k] * q8::PAGE + static_cast<int32_t>(p % q8::PAGE);
+        }
+        const int64_t i = i0 + 64 * (j >> 1) + 2 * lane, p = p0 + 64 * (j >> 1);
+        *reinterpret_cast<int2*>(a.slots + i) = make_int2(slot[0], slot[1]);
+        *reinterpret_cast<longlong2*>(a.positions + i) = make_longlong2(p, p + 1);
+      }
+      continue;
     }
-  }
-  if (i0 + TPT <= n && (reinterpret_cast<uintptr_t>(a.slots) & 15) == 0 &&
-      (reinterpret_cast<uintptr_t>(a.positions) & 15) == 0) {
-#pragma unroll
-    for (int j = 0; j < TPT; j += 4)
-      *reinterpret_cast<int4*>(a.slots + i0 + j) = make_int4(slot[j], slot[j + 1], slot[j + 2], slot[j + 3]);
-#pragma unroll
-    for (int j = 0; j < TPT; j += 2)
-      *reinterpret_cast<longlong2*>(a.positions + i0 + j) = make_longlong2(pos[j], pos[j + 1]);
-  } else {
-#pragma unroll
-    for (int j = 0; j < TPT; ++j)
-      if (i0 + j < n) {
-        a.slots[i0 + j] = slot[j];
-        a.positions[i0 + j] = pos[j];
+    int x = s;  // this lane's session
+    int64_t xb = begin, xe = end;
+#pragma unroll 1
+    for (int j = 0; j < TPT; ++j) {
+      const int64_t i = i0 + 32 * j + lane;
+      if (i >= i1) break;
+      while (i >= xe && x + 1 < S) {
+        ++x;
+        xb = xe;
+        xe = q_start[x + 1];
       }
+      int32_t slot = -1, pos = -1;  // positions fit: a table row holds fewer than 2^31 tokens
+      const int32_t have = held_of(x);
+      if (i < xe && have >= 0) {
+        pos = have + static_cast<int32_t>(i - xb);
+        const int32_t idx = pos / q8::PAGE, held = pages_of(have);
+        int32_t* row = a.block_table + static_cast<int64_t>(x) * a.width;
+        const int32_t page = idx < held ? row[idx] : a.free_pages[top - 1 - (rank_of(x) + idx - held)];
+        if (idx >= held && pos % q8::PAGE == 0) row[idx] = page;  // a new page's first token enters it
+        slot = page < 0 ? -1 : page * q8::PAGE + pos % q8::PAGE;
+      }
+      a.slots[i] = slot;
+      a.positions[i] = pos;
+    }
   }
 }
 
+// `fused`: the sessions fit one pass of the threads and the tokens are
+// finished here, from shared memory.
 __global__ void __launch_bounds__(PT) plan_rows_kernel(const ic_page_plan_args a, int fused) {
   __shared__ int64_t warp_sums[32];
+  __shared__ int32_t taken_s;
+  __shared__ int32_t qs[PT + 1], len_s[PT], rank_s[PT];
+  if (threadIdx.x == 0) taken_s = 0;
   grid_dependency_wait();
   grid_launch_dependents();
   const int S = a.num_sessions;
@@ -127,8 +151,9 @@ __global__ void __launch_bounds__(PT) plan_rows_kernel(const ic_page_plan_args a
     bad = true;
     top = 0;
   }
-  int64_t tokens = 0, pages = 0, taken = 0;
-  for (int s0 = 0; s0 < S; s0 += PT) {
+  int64_t tokens = 0, pages = 0;
+  int32_t taken = 0;  // pages up to the last granted one: grants are a prefix of the needs
+  for (int s0 = 0; s0 < S; s0 += blockDim.x) {
     const int s = s0 + threadIdx.x;
     const int64_t len = s < S ? a.lens[s] : 0;
     const int64_t c = s < S ? a.counts[s] : 0;
@@ -140,33 +165,49 @@ __global__ void __launch_bounds__(PT) plan_rows_kernel(const ic_page_plan_args a
     const int64_t upto = pages + block_scan(need, warp_sums, sum);
     pages += sum;
     const bool granted = fits && (need == 0 || upto <= top);
-    block_scan(granted ? need : 0, warp_sums, sum);
-    taken += sum;
+    if (granted && need > 0) taken = static_cast<int32_t>(upto);
     if (s < S) {
-      a.q_start[s + 1] = static_cast<int32_t>(q_end < 0x7fffffff ? q_end : 0x7fffffff);
-      a.workspace[2 * s] = granted ? static_cast<int32_t>(len) : -1;
-      a.workspace[2 * s + 1] = static_cast<int32_t>(upto - need);
+      const int32_t q_to = static_cast<int32_t>(q_end < 0x7fffffff ? q_end : 0x7fffffff);
+      const int32_t had = granted ? static_cast<int32_t>(len) : -1, rank = static_cast<int32_t>(upto - need);
+      a.q_start[s + 1] = q_to;
+      if (fused) {
+        qs[s + 1] = q_to;
+        len_s[s] = had;
+        rank_s[s] = rank;
+      } else {
+        a.workspace[2 * s] = had;
+        a.workspace[2 * s + 1] = rank;
+      }
       a.lens_out[s] = static_cast<int32_t>(granted ? len + c : len);
       bad |= !granted;
     }
   }
   if (threadIdx.x == 0) {
     a.q_start[0] = 0;
+    qs[0] = 0;
     a.workspace[2 * S] = top;
-    *a.free_count_out = top - static_cast<int32_t>(taken);
   }
+  taken = __reduce_max_sync(FULL_MASK, taken);
+  if ((threadIdx.x & 31) == 0 && taken > 0) atomicMax(&taken_s, taken);
   if (__syncthreads_or(bad) && threadIdx.x == 0 && a.dev_status) atomicOr(a.dev_status, IC_DEVFLAG_NO_PAGES);
-  if (fused) plan_tokens(a, a.q_start, a.workspace, static_cast<int64_t>(threadIdx.x) * TPT);
+  if (threadIdx.x == 0) *a.free_count_out = top - taken_s;
+  if (fused) {
+    const int64_t i0 = static_cast<int64_t>(threadIdx.x >> 5) * WT;
+    plan_tokens(a, qs, len_s, rank_s, 1, top, i0, min(i0 + WT, static_cast<int64_t>(a.total)));
+  }
 }
 
-__global__ void __launch_bounds__(256) plan_tokens_kernel(const ic_page_plan_args a) {
-  extern __shared__ int32_t qs[];  // q_start, when it fits
+// Each warp takes `per_warp` consecutive tokens (a multiple of WT).
+__global__ void __launch_bounds__(256) plan_tokens_kernel(const ic_page_plan_args a, int64_t per_warp) {
+  extern __shared__ int32_t qs[];
   grid_dependency_wait();
   grid_launch_dependents();
   const int S = a.num_sessions;
   for (int s = threadIdx.x; s <= S; s += blockDim.x) qs[s] = a.q_start[s];
   __syncthreads();
-  plan_tokens(a, qs, a.workspace, (static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x) * TPT);
+  const int64_t i0 = (static_cast<int64_t>(blockIdx.x) * (blockDim.x >> 5) + (threadIdx.x >> 5)) * per_warp;
+  plan_tokens(a, qs, a.workspace, a.workspace + 1, 2, a.workspace[2 * S], i0,
+              min(i0 + per_warp, static_cast<int64_t>(a.total)));
 }
 
 __global__ void __launch_bounds__(PT) release_kernel(const ic_page_release_args a) {
@@ -235,15 +276,22 @@ extern "C" int ic_page_plan(const ic_page_plan_args* a, void* stream) {
   }
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   ic_page_plan_args args = *a;
-  int fused = a->total <= ic::FUSED_TOKENS ? 1 : 0;
+  int fused = a->total <= ic::FUSED_TOKENS && a->num_sessions <= ic::PT ? 1 : 0;
+  // no more warps than the sessions and, when fused, the tokens need: barriers
+  // and scans over idle warps would be most of a decode tick's plan
+  int threads = a->num_sessions < ic::PT ? (a->num_sessions + 31) / 32 * 32 : ic::PT;
+  if (fused) threads = max(threads, (a->total + ic::WT - 1) / ic::WT * 32);
   void* p1[] = {&args, &fused};
-  int rc = ic::launch_pdl(reinterpret_cast<const void*>(ic::plan_rows_kernel), dim3(1), dim3(ic::PT), 0, st, p1,
+  int rc = ic::launch_pdl(reinterpret_cast<const void*>(ic::plan_rows_kernel), dim3(1), dim3(threads), 0, st, p1,
                           "page_plan (sessions)");
   if (rc != IC_OK || fused) return rc;
-  const int64_t threads = (static_cast<int64_t>(a->total) + ic::TPT - 1) / ic::TPT;
-  void* p2[] = {&args};
+  // one wave of 8 CTAs per SM at most: a CTA copies q_start before it begins
+  const int64_t warps = static_cast<int64_t>(148) * 8 * 8;
+  int64_t per_warp = ((a->total + warps - 1) / warps + ic::WT - 1) / ic::WT * ic::WT;
+  const int64_t per_cta = 8 * per_warp;
+  void* p2[] = {&args, &per_warp};
   return ic::launch_pdl(reinterpret_cast<const void*>(ic::plan_tokens_kernel),
-                        dim3(static_cast<unsigned>((threads + 255) / 256)), dim3(256), (a->num_sessions + 1) * 4, st, p2,
+                        dim3(static_cast<unsigned>((a->total + per_cta - 1) / per_cta)), dim3(256), (a->num_sessions + 1) * 4, st, p2,
                         "page_plan (tokens)");
 }
 

@@ -5,9 +5,12 @@
 // into registers, their largest magnitude gives the page scale's exponent, and
 // the codes are stored; a run that does not start its page and needs a larger
 // scale first rounds the page's other codes again.  Read: one thread per
-// 8 codes.  Both are bound by HBM: a write moves size + 1 bytes per element, a
-// read 1 + size.
+// 8 codes of RT tokens.  Both are bound by HBM (a write moves size + 1 bytes per
+// element, a read 1 + size) as long as an element costs few instructions, which
+// is why maxima and fp16 codes are taken two at a time.
 #include <stdio.h>
+
+#include <type_traits>
 
 #include "common.cuh"
 #include "launch.cuh"
@@ -48,62 +51,139 @@ __device__ __forceinline__ int64_t slot_of(const Range& r, int64_t t) {
   return page < 0 ? -1 : static_cast<int64_t>(page) * q8::PAGE + lt % q8::PAGE;
 }
 
-// 4 source elements as floats from their raw bits.
-template <typename T> struct Raw4;
-template <> struct Raw4<float> {
-  using type = uint4;
-  __device__ static void floats(const uint4& u, float* o) {
-    o[0] = __uint_as_float(u.x); o[1] = __uint_as_float(u.y); o[2] = __uint_as_float(u.z); o[3] = __uint_as_float(u.w);
+// A lane's vector of a source row: 16 bytes.
+template <typename T> constexpr int VE = 16 / sizeof(T);
+
+__device__ __forceinline__ void vec_floats(const uint4& u, float* o, const float*) {
+  o[0] = __uint_as_float(u.x); o[1] = __uint_as_float(u.y); o[2] = __uint_as_float(u.z); o[3] = __uint_as_float(u.w);
+}
+template <typename T>
+__device__ __forceinline__ void vec_floats(const uint4& u, float* o, const T*) {
+  const uint2 lo = make_uint2(u.x, u.y), hi = make_uint2(u.z, u.w);
+  load4(reinterpret_cast<const T*>(&lo), o);
+  load4(reinterpret_cast<const T*>(&hi), o + 4);
+}
+
+// The largest magnitude among vectors, kept as the type's own bits (two 16-bit
+// maxima per register): as unsigned integers they order like the magnitudes,
+// with infinities and NaN above every finite value.
+template <typename T>
+__device__ __forceinline__ uint32_t max_bits(uint32_t m, const uint4& u) {
+  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    m = sizeof(T) == 4 ? max(m, w[i] & 0x7fffffffu) : __vmaxu2(m, w[i] & 0x7fff7fffu);
+  return m;
+}
+// The warp's maximum as the bits of a float (>= 0x7f800000: not finite).
+__device__ __forceinline__ uint32_t warp_max_bits(uint32_t m, const float*) { return __reduce_max_sync(FULL_MASK, m); }
+__device__ __forceinline__ uint32_t warp_max_bits(uint32_t m, const __nv_bfloat16*) {
+  return __reduce_max_sync(FULL_MASK, max(m & 0xffffu, m >> 16)) << 16;
+}
+__device__ __forceinline__ uint32_t warp_max_bits(uint32_t m, const __half*) {
+  const uint32_t h = __reduce_max_sync(FULL_MASK, max(m & 0xffffu, m >> 16));
+  return __float_as_uint(__half2float(__ushort_as_half(static_cast<uint16_t>(h))));
+}
+
+// Codes of one vector whose values are finite and at most QMAX * 2^e, four per
+// word.  int8: adding 1.5 * 2^23 rounds to nearest even and leaves the integer
+// in the low byte; e4m3: the conversion instruction.
+template <int CODE, typename T>
+__device__ __forceinline__ void encode_vec(const uint4& u, int e, uint32_t* o, const T* type) {
+  const float unit = q8::two_to(-e);
+  float x[VE<T>];
+  vec_floats(u, x, type);
+#pragma unroll
+  for (int i = 0; i < VE<T> / 4; ++i) {
+    if (CODE == IC_E4M3) {
+      uint16_t lo, hi;
+      asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(lo) : "f"(x[4 * i + 1] * unit), "f"(x[4 * i] * unit));
+      asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(hi) : "f"(x[4 * i + 3] * unit), "f"(x[4 * i + 2] * unit));
+      o[i] = static_cast<uint32_t>(lo) | (static_cast<uint32_t>(hi) << 16);
+    } else {
+      uint32_t r[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) r[k] = __float_as_uint(fmaf(x[4 * i + k], unit, 12582912.f));
+      o[i] = __byte_perm(__byte_perm(r[0], r[1], 0x0040), __byte_perm(r[2], r[3], 0x0040), 0x5410);
+    }
   }
-};
-template <> struct Raw4<__half> {
-  using type = uint2;
-  __device__ static void floats(const uint2& u, float* o) { load4(reinterpret_cast<const __half*>(&u), o); }
-};
-template <> struct Raw4<__nv_bfloat16> {
-  using type = uint2;
-  __device__ static void floats(const uint2& u, float* o) { load4(reinterpret_cast<const __nv_bfloat16*>(&u), o); }
-};
+}
+// fp16 sources whose unit is an fp16 number stay in fp16, two values an
+// instruction: the product with a power of two and the addition of 1.5 * 2^10
+// round once (a product that turns subnormal lies far under half a code step).
+template <int CODE>
+__device__ __forceinline__ void encode_half(const uint4& u, __half2 unit, uint32_t* o) {
+  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const __half2 a = *reinterpret_cast<const __half2*>(&w[2 * i]), b = *reinterpret_cast<const __half2*>(&w[2 * i + 1]);
+    if (CODE == IC_E4M3) {
+      __half2 x = __hmul2(a, unit), y = __hmul2(b, unit);
+      uint16_t lo, hi;
+      asm("cvt.rn.satfinite.e4m3x2.f16x2 %0, %1;" : "=h"(lo) : "r"(*reinterpret_cast<uint32_t*>(&x)));
+      asm("cvt.rn.satfinite.e4m3x2.f16x2 %0, %1;" : "=h"(hi) : "r"(*reinterpret_cast<uint32_t*>(&y)));
+      o[i] = static_cast<uint32_t>(lo) | (static_cast<uint32_t>(hi) << 16);
+    } else {
+      const __half2 off = __float2half2_rn(1536.f);
+      __half2 x = __hfma2(a, unit, off), y = __hfma2(b, unit, off);
+      o[i] = __byte_perm(*reinterpret_cast<uint32_t*>(&x), *reinterpret_cast<uint32_t*>(&y), 0x6420);
+    }
+  }
+}
+
+template <int N>
+__device__ __forceinline__ void store_codes(uint32_t* dst, const uint32_t* o) {
+  if (N == 2)
+    *reinterpret_cast<uint2*>(dst) = make_uint2(o[0], o[1]);
+  else
+    *dst = o[0];
+}
 
 // `cnt` tokens, source rows src + t * stride (elements), into slots off ..
 // off + cnt - 1 of the page at `page` (16 rows of D codes).
 template <typename T, int D, int CODE>
 __device__ __forceinline__ void write_run(const T* src, int64_t stride, int cnt, int off, uint8_t* page, float* scale_p,
                                           int32_t* status, int lane) {
-  constexpr int V4 = D / 4;                   // 4-element vectors per row
-  constexpr int NV = q8::PAGE * V4 / 32;      // vectors per lane for a whole page
-  using R = typename Raw4<T>::type;
-  R raw[NV];
+  constexpr int E = VE<T>, W = E / 4;         // elements and code words per vector
+  constexpr int VR = D / E;                   // vectors per row
+  constexpr int NV = q8::PAGE * VR / 32;      // vectors per lane for a whole page
+  const T* type = nullptr;
+  uint4 raw[NV];
 #pragma unroll
   for (int j = 0; j < NV; ++j) {
-    const int it = lane + 32 * j, t = it / V4, c = it % V4;
-    raw[j] = R{};
-    if (t < cnt) raw[j] = *reinterpret_cast<const R*>(src + t * stride + 4 * c);
+    const int it = lane + 32 * j, t = it / VR;
+    raw[j] = make_uint4(0, 0, 0, 0);
+    if (t < cnt) raw[j] = reinterpret_cast<const uint4*>(src + t * stride)[it % VR];
   }
   const float held = off > 0 ? *scale_p : 0.f;
-  uint32_t amax = 0;
-  bool odd = false;
+  uint32_t m = 0;
 #pragma unroll
-  for (int j = 0; j < NV; ++j) {
-    float x[4];
-    Raw4<T>::floats(raw[j], x);
+  for (int j = 0; j < NV; ++j) m = max_bits<T>(m, raw[j]);
+  uint32_t amax = warp_max_bits(m, type);
+  bool plain = amax < 0x7f800000u;            // every value finite
+  if (!plain) {
+    amax = 0;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const uint32_t b = __float_as_uint(x[i]) & 0x7fffffffu;
-      const bool finite = b < 0x7f800000u;
-      odd |= !finite;
-      amax = max(amax, finite ? b : 0u);
+    for (int j = 0; j < NV; ++j) {
+      float x[E];
+      vec_floats(raw[j], x, type);
+#pragma unroll
+      for (int i = 0; i < E; ++i) {
+        const uint32_t b = __float_as_uint(x[i]) & 0x7fffffffu;
+        amax = max(amax, b < 0x7f800000u ? b : 0u);
+      }
     }
+    amax = __reduce_max_sync(FULL_MASK, amax);
+    if (lane == 0 && status) atomicOr(status, IC_DEVFLAG_NONFINITE);
   }
-  amax = __reduce_max_sync(FULL_MASK, amax);
-  if (__any_sync(FULL_MASK, odd) && lane == 0 && status) atomicOr(status, IC_DEVFLAG_NONFINITE);
   int e = q8::exponent_for<CODE>(amax);
+  if (e == q8::E_MAX) plain = false;          // the values may pass the largest code
   if (off > 0) {
     const int e_old = static_cast<int>((__float_as_uint(held) >> 23) & 255u) - 127;
     if (e > e_old) {  // round the page's other codes again to the larger unit
       const float f = q8::two_to(max(e_old - e, -126));
-      for (int it = lane; it < q8::PAGE * V4; it += 32) {
-        const int t = it / V4;
+      for (int it = lane; it < q8::PAGE * D / 4; it += 32) {
+        const int t = it / (D / 4);
         if (t >= off && t < off + cnt) continue;
         uint32_t* p = reinterpret_cast<uint32_t*>(page) + it;
         float x[4];
@@ -114,14 +194,36 @@ __device__ __forceinline__ void write_run(const T* src, int64_t stride, int cnt,
       e = q8::clamp_exp(e_old);
     }
   }
-  const float unit = q8::two_to(-e);
+  uint32_t* dst = reinterpret_cast<uint32_t*>(page + off * D);
+  if (plain && sizeof(T) == 2 && std::is_same<T, __half>::value && e >= -15 && e <= 24) {
+    const __half2 unit = __float2half2_rn(q8::two_to(-e));
 #pragma unroll
-  for (int j = 0; j < NV; ++j) {
-    const int it = lane + 32 * j, t = it / V4;
-    if (t < cnt) {
-      float x[4];
-      Raw4<T>::floats(raw[j], x);
-      reinterpret_cast<uint32_t*>(page + off * D)[it] = q8::encode4<CODE>(x[0] * unit, x[1] * unit, x[2] * unit, x[3] * unit);
+    for (int j = 0; j < NV; ++j) {
+      const int it = lane + 32 * j;
+      uint32_t o[2];
+      encode_half<CODE>(raw[j], unit, o);
+      if (it / VR < cnt) store_codes<W>(dst + it * W, o);
+    }
+  } else if (plain) {
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      const int it = lane + 32 * j;
+      uint32_t o[W];
+      encode_vec<CODE>(raw[j], e, o, type);
+      if (it / VR < cnt) store_codes<W>(dst + it * W, o);
+    }
+  } else {
+    const float unit = q8::two_to(-e);
+#pragma unroll 1
+    for (int j = 0; j < NV; ++j) {
+      const int it = lane + 32 * j, t = it / VR;
+      if (t >= cnt) break;
+      const uint4 u = reinterpret_cast<const uint4*>(src + t * stride)[it % VR];
+      float x[E];
+      vec_floats(u, x, type);
+#pragma unroll
+      for (int i = 0; i < W; ++i)
+        dst[it * W + i] = q8::encode4<CODE>(x[4 * i] * unit, x[4 * i + 1] * unit, x[4 * i + 2] * unit, x[4 * i + 3] * unit);
     }
   }
   __syncwarp();  // every lane has read the old scale
@@ -179,49 +281,82 @@ __global__ void __launch_bounds__(WARPS * 32) write_kernel(const __grid_constant
   }
 }
 
-template <typename T>
-__device__ __forceinline__ void store8(T* p, const float* x, float s) {
-  uint32_t u[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    T lo = DT<T>::from_f(x[2 * i] * s), hi = DT<T>::from_f(x[2 * i + 1] * s);
-    u[i] = static_cast<uint32_t>(*reinterpret_cast<uint16_t*>(&lo)) |
-           (static_cast<uint32_t>(*reinterpret_cast<uint16_t*>(&hi)) << 16);
-  }
-  *reinterpret_cast<uint4*>(p) = make_uint4(u[0], u[1], u[2], u[3]);
+// 8 codes times their scale 2^e, rounded once to T.
+__device__ __forceinline__ uint32_t pack_pair(float a, float b, const __half*) {
+  const __half2 h = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
 }
-template <>
-__device__ __forceinline__ void store8<float>(float* p, const float* x, float s) {
+__device__ __forceinline__ uint32_t pack_pair(float a, float b, const __nv_bfloat16*) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+template <int CODE, typename T>
+__device__ __forceinline__ void store8(T* p, const uint2& u, float s) {
+  uint32_t h[4];
+  q8::decode4_h2<CODE>(u.x, h[0], h[1]);
+  q8::decode4_h2<CODE>(u.y, h[2], h[3]);
+  if (std::is_same<T, __half>::value && s >= 6.103515625e-05f && s <= 32768.f) {  // the scale is a normal fp16 number
+    const __half2 s2 = __float2half2_rn(s);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const __half2 v = __hmul2(*reinterpret_cast<__half2*>(&h[i]), s2);
+      h[i] = *reinterpret_cast<const uint32_t*>(&v);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 v = __half22float2(*reinterpret_cast<__half2*>(&h[i]));
+      h[i] = pack_pair(v.x * s, v.y * s, p);
+    }
+  }
+  *reinterpret_cast<uint4*>(p) = make_uint4(h[0], h[1], h[2], h[3]);
+}
+template <int CODE>
+__device__ __forceinline__ void store8(float* p, const uint2& u, float s) {
+  float x[8];
+  q8::decode4<CODE>(u.x, x);
+  q8::decode4<CODE>(u.y, x + 4);
   *reinterpret_cast<float4*>(p) = make_float4(x[0] * s, x[1] * s, x[2] * s, x[3] * s);
   *reinterpret_cast<float4*>(p + 4) = make_float4(x[4] * s, x[5] * s, x[6] * s, x[7] * s);
 }
 
-template <typename T, int CODE>
-__global__ void __launch_bounds__(256) read_kernel(const __grid_constant__ Batch b, int D) {
+constexpr int RT = 4;  // tokens per thread (read): their loads are in flight together
+
+template <int D> constexpr int READ_TOKENS = RT * 256 / (D / 8);  // tokens per CTA
+
+template <typename T, int D, int CODE>
+__global__ void __launch_bounds__(256) read_kernel(const __grid_constant__ Batch b) {
+  constexpr int V8 = D / 8, STEP = 256 / V8;
   grid_dependency_wait();
   grid_launch_dependents();
-  const int64_t item = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x;
-  if (item >= b.first[b.count]) return;
   int i = 0;
-  while (b.first[i + 1] <= item) ++i;
+  while (b.first[i + 1] <= blockIdx.x) ++i;
   const Range& r = b.r[i];
-  const int v8 = D / 8;
-  const int64_t t = (item - b.first[i]) / v8;
-  const int c = static_cast<int>((item - b.first[i]) % v8);
+  const int64_t t0 = (blockIdx.x - b.first[i]) * READ_TOKENS<D> + threadIdx.x / V8;
+  const int c = threadIdx.x % V8;
   const int lh = blockIdx.y, l = lh / b.heads, h = lh % b.heads;
   const bool is_v = blockIdx.z != 0;
   const int64_t plane = static_cast<int64_t>(b.layer_begin + l) * b.heads + h;
-  T* out = reinterpret_cast<T*>(is_v ? r.v_buf : r.k_buf) + l * r.stride_l + h * r.stride_h + t * r.stride_t + 8 * c;
-  const int64_t slot = slot_of(r, t);
-  float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, s = 0.f;
-  if (slot >= 0 && slot < b.pool_tokens) {
-    const uint8_t* codes = (is_v ? b.v : b.k) + (plane * b.pool_tokens + slot) * D;
-    const uint2 u = reinterpret_cast<const uint2*>(codes)[c];
-    s = (is_v ? b.v_scale : b.k_scale)[plane * (b.pool_tokens / q8::PAGE) + slot / q8::PAGE];
-    q8::decode4<CODE>(u.x, x);
-    q8::decode4<CODE>(u.y, x + 4);
+  const uint8_t* codes = (is_v ? b.v : b.k) + plane * b.pool_tokens * D;
+  const float* scales = (is_v ? b.v_scale : b.k_scale) + plane * (b.pool_tokens / q8::PAGE);
+  T* out = reinterpret_cast<T*>(is_v ? r.v_buf : r.k_buf) + l * r.stride_l + h * r.stride_h + 8 * c;
+  uint2 u[RT];
+  float s[RT];
+  int64_t slot[RT];
+#pragma unroll
+  for (int j = 0; j < RT; ++j) slot[j] = t0 + j * STEP < r.n ? slot_of(r, t0 + j * STEP) : -1;
+#pragma unroll
+  for (int j = 0; j < RT; ++j) {
+    u[j] = make_uint2(0, 0);
+    s[j] = 0.f;
+    if (slot[j] >= 0 && slot[j] < b.pool_tokens) {
+      u[j] = reinterpret_cast<const uint2*>(codes + slot[j] * D)[c];
+      s[j] = scales[slot[j] / q8::PAGE];
+    }
   }
-  store8<T>(out, x, s);
+#pragma unroll
+  for (int j = 0; j < RT; ++j)
+    if (t0 + j * STEP < r.n) store8<CODE>(out + (t0 + j * STEP) * r.stride_t, u[j], s[j]);
 }
 
 bool q8_args_ok(const ic_page_q8_args* a, const char* name) {
@@ -291,10 +426,14 @@ template <typename T>
 const void* write_fn_d(int d, int code) {
   return d == 64 ? write_fn<T, 64>(code) : d == 128 ? write_fn<T, 128>(code) : write_fn<T, 256>(code);
 }
-template <typename T>
+template <typename T, int D>
 const void* read_fn(int code) {
-  return code == IC_E4M3 ? reinterpret_cast<const void*>(read_kernel<T, IC_E4M3>)
-                         : reinterpret_cast<const void*>(read_kernel<T, IC_I8>);
+  return code == IC_E4M3 ? reinterpret_cast<const void*>(read_kernel<T, D, IC_E4M3>)
+                         : reinterpret_cast<const void*>(read_kernel<T, D, IC_I8>);
+}
+template <typename T>
+const void* read_fn_d(int d, int code) {
+  return d == 64 ? read_fn<T, 64>(code) : d == 128 ? read_fn<T, 128>(code) : read_fn<T, 256>(code);
 }
 
 }  // namespace
@@ -340,23 +479,24 @@ extern "C" int ic_page_write_q8(const ic_page_q8_args* a, void* stream) {
 extern "C" int ic_page_read_q8(const ic_page_q8_args* a, void* stream) {
   using namespace ic;
   if (!q8_args_ok(a, "page_read_q8")) return IC_ERR_INVALID_ARG;
-  int D = a->pool.head_dim;
+  const int D = a->pool.head_dim;
   if (D != 64 && D != 128 && D != 256) return q8_dim_error("page_read_q8");
   const int planes = (a->layer_end - a->layer_begin) * a->pool.num_kv_heads;
   if (planes == 0) return IC_OK;
   Batch b = {};
   fill_batch(a, b);
-  for (int i = 0; i < a->count; ++i) b.first[i + 1] = b.first[i] + a->rows[i].n_tokens * (D / 8);
-  const int64_t blocks = (b.first[b.count] + 255) / 256;
+  const int per_cta = RT * 256 / (D / 8);
+  for (int i = 0; i < a->count; ++i) b.first[i + 1] = b.first[i] + (a->rows[i].n_tokens + per_cta - 1) / per_cta;
+  const int64_t blocks = b.first[b.count];
   if (blocks == 0) return IC_OK;
   if (blocks > 0x7fffffff) {
     set_last_error("page_read_q8: too many tokens for one launch");
     return IC_ERR_UNSUPPORTED;
   }
-  const void* fn = a->buf_dtype == IC_F32   ? read_fn<float>(a->pool.dtype)
-                   : a->buf_dtype == IC_F16 ? read_fn<__half>(a->pool.dtype)
-                                            : read_fn<__nv_bfloat16>(a->pool.dtype);
-  void* p[] = {&b, &D};
+  const void* fn = a->buf_dtype == IC_F32   ? read_fn_d<float>(D, a->pool.dtype)
+                   : a->buf_dtype == IC_F16 ? read_fn_d<__half>(D, a->pool.dtype)
+                                            : read_fn_d<__nv_bfloat16>(D, a->pool.dtype);
+  void* p[] = {&b};
   return launch_pdl(fn, dim3(static_cast<unsigned>(blocks), planes, 2), dim3(256), 0, static_cast<cudaStream_t>(stream),
                     p, "page_read_q8");
 }
