@@ -69,6 +69,20 @@ int check(const ic_paged_attn_args* a) {
   return IC_OK;
 }
 
+constexpr int ALL_ROWS = 0x7fffffff;
+
+// Sessions with at most this many query rows per KV head are the streaming
+// kernel's.  It reads a session's pages once per 16 rows, the tile kernel
+// converts them once per 256 but gives each (session, KV head, 256 rows) to one
+// CTA: below some 20 such CTAs the streaming kernel's even shares win although
+// it does the work several times over.
+int few_rows(const ic_paged_attn_args* a) {
+  const int64_t G = a->num_q_heads / a->num_kv_heads;
+  if (a->head_dim == 256 || a->max_count * G <= 64 || a->num_q_tokens * static_cast<int64_t>(a->num_q_heads) <= 4096)
+    return ALL_ROWS;
+  return 64;
+}
+
 }  // namespace
 
 int page_map(CUtensorMap* m, const void* codes, int64_t pool_tokens, int heads, int D) {
@@ -102,7 +116,7 @@ extern "C" int64_t ic_paged_attention_workspace(const ic_paged_attn_args* a) {
 
 extern "C" int ic_paged_attention(const ic_paged_attn_args* a, void* stream) {
   using namespace ic;
-  const int rc = paged::check(a);
+  int rc = paged::check(a);
   if (rc != IC_OK) return rc;
   if (!a->workspace || !paged::aligned16(a->workspace) || a->workspace_bytes < ic_paged_attention_workspace(a)) {
     set_last_error("paged_attention: workspace missing, misaligned or too small");
@@ -110,6 +124,8 @@ extern "C" int ic_paged_attention(const ic_paged_attn_args* a, void* stream) {
   }
   paged::Params p;
   p.q = a->q;
+  p.k = a->k;
+  p.v = a->v;
   p.out = a->out;
   p.lse = a->lse;
   p.table = a->block_table;
@@ -128,8 +144,10 @@ extern "C" int ic_paged_attention(const ic_paged_attn_args* a, void* stream) {
   p.G = a->num_q_heads / a->num_kv_heads;
   p.n_pages = static_cast<int32_t>(a->pool_tokens / q8::PAGE);
   p.n_q = a->num_q_tokens;
-  p.few_rows = 0x7fffffff;
+  p.few_rows = paged::few_rows(a);
   p.min_share = 16;
   p.sl2 = a->scale * paged::LOG2E;
-  return paged::launch_stream(p, *a, static_cast<cudaStream_t>(stream));
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (p.few_rows != paged::ALL_ROWS && (rc = paged::launch_tile(p, *a, st)) != IC_OK) return rc;
+  return paged::launch_stream(p, *a, st);
 }

@@ -2,6 +2,8 @@
 // sessions' row counts, tensor maps over 8-bit pages.
 #pragma once
 
+#include <algorithm>
+
 #include "common.cuh"
 #include "q8.cuh"
 
@@ -14,6 +16,8 @@ constexpr float LN2 = 0.6931471805599453f;
 
 struct Params {
   const void* q;
+  const void* k;              // codes of the layer
+  const void* v;
   void* out;
   float* lse;                 // may be null
   const int32_t* table;

@@ -320,6 +320,60 @@ def test_attention_scales_far_apart(codes):
     check_attention(x[:4] + (zero,) + x[5:])
 
 
+TILE_LENS, TILE_COUNTS = [700, 90, 40, 33, 513, 2000, 0, 160], [300, 1, 40, 0, 129, 260, 3, 160]
+
+
+@pytest.mark.parametrize("codes", CODES)
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("H,G,D", [(2, 8, 128), (1, 7, 128), (2, 5, 64), (4, 3, 128), (1, 16, 64)])
+def test_attention_prompts(codes, dtype, H, G, D):
+    """Enough query rows for the tile kernel, beside sessions that are not: chunks
+    on top of held tokens, whole prompts, ranges that end inside tiles and
+    pages, more tokens than are held."""
+    x = attention_inputs(H * G + D, TILE_LENS, TILE_COUNTS, H, G, D, codes, dtype)
+    assert x[0].shape[0] * x[0].shape[1] > 4096
+    _, _, status = check_attention(x, max_count=300)
+    assert status == 0
+    check_attention(x)
+
+
+@pytest.mark.parametrize("codes", CODES)
+def test_attention_prompts_hard_cases(codes):
+    from infercache_b200.paged_ops import paged_attention
+    x = attention_inputs(3, TILE_LENS, TILE_COUNTS, 2, 4, 128, codes, torch.bfloat16, k_spread=6, v_spread=20)
+    check_attention(x)
+    check_attention((x[0] * 1e30,) + x[1:], scale=1e-30)
+    check_attention(x, scale=-0.3)
+    zero = x[4].clone()
+    zero[:, ::2] = 0.0
+    check_attention(x[:4] + (zero,) + x[5:])
+    t = x[5].clone()
+    t[0, 2], t[5, 9] = -1, 10 ** 9
+    assert check_attention(x[:5] + (t,) + x[6:])[2] == BAD_ROW
+    # strided queries, rows behind the last session, a NaN that stays in its row
+    n = x[0].shape[0]
+    wide = torch.zeros(n + 9, 8 * 128 + 64, dtype=torch.bfloat16, device="cuda")
+    wide[:n, :1024] = x[0].reshape(n, 1024)
+    view, out = wide[:, :1024].view(n + 9, 8, 128), torch.full((n + 9, 8, 128), 3.0, dtype=torch.bfloat16, device="cuda")
+    paged_attention(view, *x[1:], out=out)
+    want = paged_attention(*x)
+    assert torch.equal(out[:n], want) and bool((out[n:] == 3).all())
+    q = x[0].clone()
+    q[17, 3, 40] = math.nan
+    got = paged_attention(q, *x[1:])
+    assert bool(torch.isnan(got[17, 3]).all())
+    got[17, 3] = want[17, 3]
+    assert torch.equal(got, want)
+
+
+def test_attention_many_sessions_of_prompts():
+    """More sessions than one pass of a CTA's threads looks through."""
+    rng = np.random.default_rng(1)
+    lens = rng.integers(1, 60, 700).tolist()
+    counts = [min(n, int(c)) for n, c in zip(lens, rng.integers(0, 40, 700))]
+    check_attention(attention_inputs(2, lens, counts, 1, 4, 64, torch.int8, torch.float16))
+
+
 def test_attention_strides_padding_and_out():
     from infercache_b200.paged_ops import paged_attention
     q, k, v, ks, vs, table, lens, q_start = attention_inputs(8, [70, 20], [2, 1], 2, 4, 64, torch.int8, torch.float16)
