@@ -8,7 +8,7 @@
 // tile, so a key's codes are converted once per 256 rows.  Roles:
 //   warpgroup 0  warp 0 issues S = Q K^T (tcgen05.mma, fp16 operands in shared
 //                memory, fp32 in TMEM), warp 1 issues O += P V (P read from TMEM);
-//   warpgroup 1  loads the pages' codes (16 bytes a lane, one key tile ahead in
+//   warpgroup 1  loads the pages' codes (16 bytes a lane, two tiles ahead in
 //                registers), converts them to fp16 -- exact for both formats --
 //                and stores them as 128-byte-swizzled operand tiles into a ring,
 //                in consumption order K0 K1 V0 K2 V1 ..., with the pages' scales
@@ -20,7 +20,14 @@
 //                O rescaled only when u passes M by more than 8.
 // The V scales sit in the exponent for the reason given in paged_stream.cu.
 // The score tiles take turns in one TMEM buffer: each row copies its scores to
-// registers at once, so the next Q K^T overlaps its exponentials.
+// registers at once, so the next Q K^T overlaps its exponentials.  P is handed
+// over in two halves of 64 keys.
+// Measured (4 sessions x 1500-2048 tokens x 16 heads over 4096-8192 keys, D =
+// 128, e4m3): 1.9 us per step of two query tiles x 128 keys, of which the tensor
+// cores need 1.1, plus about 10 us per CTA to begin and end.  Codes loaded one
+// tile ahead instead of two, 325 us a call instead of 285; a pass of its own
+// for the scores' scaling, no change; two score buffers with P in the scores'
+// place, 337 us against 327 at the time.
 // TMEM columns: S 0, P_a 128, P_b 192, O_a 256, O_b 384.  Registers: 512
 // threads start with 128 each; warpgroups 0 and 1 give theirs to the softmax
 // (56 + 96 + 176 + 176 = 504 of 512).
@@ -46,6 +53,7 @@ constexpr int SUB = TB * 64 * 2;       // one 64-column swizzled sub-tile: 16 KB
 constexpr int THREADS = 512;
 constexpr int RS = 5;                  // K / V ring slots
 constexpr int NSC = 8;                 // key tiles whose scales are kept: the ring runs at most 3 ahead of the softmax
+constexpr int SORTED = 128;            // up to this many sessions are taken longest first
 constexpr float SLACK = 8.f, LIFT = 7.f;
 
 template <int D>
@@ -53,8 +61,8 @@ struct Lay {
   static constexpr int TILE = D / 64 * SUB;
   static constexpr int RING = 2 * TILE;
   static constexpr int SCALES = RING + RS * TILE;      // [NSC][3][8]: k scale, log2 v scale, 1 / v scale
-  static constexpr int BARS = SCALES + NSC * 24 * 4;
-  static constexpr int NBAR = 20;
+  static constexpr int BARS = SCALES + NSC * 24 * 4;   // 16-byte aligned rows of 8
+  static constexpr int NBAR = 22;
   static constexpr int MISC = BARS + NBAR * 8;         // TMEM address, abort, session, pair; the scan's 16 sums
   static constexpr int BYTES = MISC + 16 + 64 + 1024;  // + alignment
 };
@@ -84,6 +92,12 @@ __device__ __forceinline__ void sts128(uint32_t addr, uint32_t x, uint32_t y, ui
   asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
 }
 
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+
 template <typename QT, int D, int CODE>
 __global__ void __launch_bounds__(THREADS, 1) tile_kernel(const Params p) {
   using L = Lay<D>;
@@ -98,34 +112,71 @@ __global__ void __launch_bounds__(THREADS, 1) tile_kernel(const Params p) {
   uint64_t* r_empty = bars + 6;   // [RS]
   uint64_t* s_full = bars + 11;   // [2]
   uint64_t* s_free = bars + 13;
-  uint64_t* p_full = bars + 14;   // [2]
-  uint64_t* pv_done = bars + 16;  // [2]
-  uint64_t* mma_done = bars + 18;
+  uint64_t* p_full = bars + 14;   // [2][2]: tile, half of its keys
+  uint64_t* pv_done = bars + 18;  // [2]
+  uint64_t* mma_done = bars + 20;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + L::MISC);
   volatile int* abort = reinterpret_cast<volatile int*>(smem + L::MISC + 4);
   volatile int* found = reinterpret_cast<volatile int*>(smem + L::MISC + 8);  // session, pair
   int* sums = reinterpret_cast<int*>(smem + L::MISC + 16);
+  int2* sorted = reinterpret_cast<int2*>(smem + L::RING);  // before the ring is written
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
   if (tid == 0) {
     *abort = 0;
     found[0] = -1;
+    mbar_init(q_full, 256);
+    for (int i = 0; i < RS; ++i) {
+      mbar_init(r_full + i, 128);
+      mbar_init(r_empty + i, 1);
+    }
+    for (int x = 0; x < 2; ++x) {
+      mbar_init(s_full + x, 1);
+      mbar_init(p_full + 2 * x, 128);
+      mbar_init(p_full + 2 * x + 1, 128);
+      mbar_init(pv_done + x, 1);
+    }
+    mbar_init(s_free, 128);
+    mbar_init(mma_done, 2);
+    fence_barrier_init();
   }
+  if (warp == 0) tc::tmem_alloc(tmem_slot, 512);
   grid_dependency_wait();
   grid_launch_dependents();
 
   // ---- which session and pair of tiles -------------------------------------------
+  // A few sessions are taken longest first (the CTAs that run last then are the
+  // short ones), many in their order.
   const int h = blockIdx.x % p.H, unit = blockIdx.x / p.H;
-  {
+  const auto pairs_of = [&](int x) {
+    int begin;
+    const int rows = query_tokens(p, x, begin) * p.G;
+    return rows > p.few_rows ? (rows + 2 * TB - 1) / (2 * TB) : 0;
+  };
+  if (p.S <= SORTED) {
+    int own = 0, held = 0;
+    if (tid < p.S) {
+      own = pairs_of(tid);
+      held = held_tokens(p, tid);
+      sorted[tid] = make_int2(held, own);
+    }
+    __syncthreads();
+    int before = 0;
+    for (int t = 0; t < p.S; ++t) {
+      const int2 o = sorted[t];
+      if (o.x > held || (o.x == held && t < tid)) before += o.y;
+    }
+    const int at = unit - before;
+    if (tid < p.S && at >= 0 && at < own) {
+      found[0] = tid;
+      found[1] = own - 1 - at;
+    }
+    __syncthreads();
+  } else {
     int carry = 0;
     for (int s0 = 0; s0 < p.S; s0 += THREADS) {
       const int s = s0 + tid;
-      int own = 0;
-      if (s < p.S) {
-        int begin;
-        const int rows = query_tokens(p, s, begin) * p.G;
-        own = rows > p.few_rows ? (rows + 2 * TB - 1) / (2 * TB) : 0;
-      }
+      const int own = s < p.S ? pairs_of(s) : 0;
       int upto = own;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
@@ -148,8 +199,15 @@ __global__ void __launch_bounds__(THREADS, 1) tile_kernel(const Params p) {
       if (found[0] >= 0) break;
     }
   }
+  tc::fence_before();
+  __syncthreads();
+  tc::fence_after();
+  const uint32_t tmem = *tmem_slot;
   const int s = found[0], pair = found[1];
-  if (s < 0) return;
+  if (s < 0) {  // more CTAs than units: the launch counts with the most that there can be
+    if (warp == 0) tc::tmem_dealloc(tmem, 512);
+    return;
+  }
   int q_begin;
   const int n_tok = query_tokens(p, s, q_begin), rows = n_tok * p.G, len = held_tokens(p, s);
   const int row_a = pair * 2 * TB;
@@ -163,27 +221,6 @@ __global__ void __launch_bounds__(THREADS, 1) tile_kernel(const Params p) {
   const int n = has_b ? nb : na;
   const auto u_k = [&](int j) { return j == 0 ? 0 : 2 * j - 1; };
   const auto u_v = [&](int j) { return j == n - 1 ? 2 * n - 1 : 2 * j + 2; };
-
-  if (tid == 0) {
-    mbar_init(q_full, has_b ? 256 : 128);
-    for (int i = 0; i < RS; ++i) {
-      mbar_init(r_full + i, 128);
-      mbar_init(r_empty + i, 1);
-    }
-    for (int x = 0; x < 2; ++x) {
-      mbar_init(s_full + x, 1);
-      mbar_init(p_full + x, 128);
-      mbar_init(pv_done + x, 1);
-    }
-    mbar_init(s_free, 128);
-    mbar_init(mma_done, 2);
-    fence_barrier_init();
-  }
-  if (warp == 0) tc::tmem_alloc(tmem_slot, 512);
-  tc::fence_before();
-  __syncthreads();
-  tc::fence_after();
-  const uint32_t tmem = *tmem_slot;
 
   if (warp < 4) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
@@ -222,12 +259,15 @@ __global__ void __launch_bounds__(THREADS, 1) tile_kernel(const Params p) {
         const uint32_t sv = sbase + L::RING + (u % RS) * L::TILE;
         for (int x = 0; x < 2; ++x) {
           if (j >= (x ? nb : na)) continue;
-          if (!(ok = one_wait(p_full + x, j & 1, p.status, abort))) break;
-          tc::fence_after();
+          for (int half = 0; half < 2; ++half) {
+            if (!(ok = one_wait(p_full + 2 * x + half, j & 1, p.status, abort))) break;
+            tc::fence_after();
 #pragma unroll
-          for (int kk = 0; kk < TB / 16; ++kk)
-            tc::mma_ts(tmem + 256 + x * 128, tmem + 128 + x * 64 + kk * 8, mndesc(sv, kk), IDESC_PV,
-                       (j > 0 || kk > 0) ? 1u : 0u);
+            for (int kk = 0; kk < TB / 32; ++kk)
+              tc::mma_ts(tmem + 256 + x * 128, tmem + 128 + x * 64 + half * 32 + kk * 8, mndesc(sv, 4 * half + kk), IDESC_PV,
+                         (j > 0 || half > 0 || kk > 0) ? 1u : 0u);
+          }
+          if (!ok) break;
           tc::commit(pv_done + x);
         }
         if (ok) tc::commit(r_empty + u % RS);
@@ -266,80 +306,93 @@ __global__ void __launch_bounds__(THREADS, 1) tile_kernel(const Params p) {
         }
       }
     };
-    const auto load = [&](int u, const int* id, uint4 (*reg)[NS], float& ks, float& vs) {
+    // Two ring positions' codes stay in registers (positions alternate between
+    // them); as soon as a vector is stored, the one two positions on is loaded in
+    // its place, so a load has two tiles' time to arrive.
+    struct Held {
+      uint4 reg[4][NS];
+      float ks, vs;   // lanes 0, 1: the scales of pages 2 cw, 2 cw + 1 ...
+      bool mine;      // ... and whether there is such a page
+    };
+    const uint32_t lane_codes = t8 * D + c4 * 16;
+    // One page's four vectors (two groups of 8 tokens): where this lane's part of
+    // it begins, and whether every token of it is held.
+    struct At {
+      const uint8_t* ptr;
+      int tokens;   // of the page that are held: 16 but for the last page, 0 for none
+    };
+    const auto page_at = [&](int u, const int* id, int i) -> At {
       int j;
       const uint8_t* codes = what(u, j) ? vc : kc;
-#pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        const int page = id[g >> 1], tok = (g & 1) * 8 + t8;
-        const bool ok = page >= 0 && (j * 8 + cw * 2 + (g >> 1)) * q8::PAGE + tok < len;
-#pragma unroll
-        for (int sub = 0; sub < NS; ++sub) {
-          reg[g][sub] = make_uint4(0, 0, 0, 0);
-          if (ok)
-            reg[g][sub] = *reinterpret_cast<const uint4*>(codes + (static_cast<int64_t>(page) * q8::PAGE + tok) * D +
-                                                          sub * 64 + c4 * 16);
-        }
-      }
-      ks = 0.f;
-      vs = 0.f;
-      if (lane < 2 && id[lane & 1] >= 0) {
-        ks = p.k_scale[plane + id[lane & 1]];
-        vs = p.v_scale[plane + id[lane & 1]];
+      const int left = len - (j * 8 + cw * 2 + i) * q8::PAGE;
+      return At{codes + static_cast<int64_t>(max(id[i], 0)) * (q8::PAGE * D) + lane_codes, id[i] < 0 ? 0 : min(left, q8::PAGE)};
+    };
+    const auto load_one = [&](const At& at, int g, int sub) -> uint4 {
+      if (at.tokens < q8::PAGE && (g & 1) * 8 + t8 >= at.tokens) return make_uint4(0, 0, 0, 0);
+      return *reinterpret_cast<const uint4*>(at.ptr + (g & 1) * 8 * D + sub * 64);
+    };
+    const auto load_scales = [&](const int* id, Held& b) {
+      const int page = id[lane & 1];
+      b.mine = lane < 2 && page >= 0;
+      b.ks = b.vs = 1.f;
+      if (b.mine) {
+        b.ks = p.k_scale[plane + page];
+        b.vs = p.v_scale[plane + page];
       }
     };
-    uint4 cur[4][NS], nxt[4][NS];
-    int id1[2], id2[2];
-    float ks, vs, ksn, vsn;
-    bool mine;   // whether this lane's page (lanes 0, 1) can be attended
-    bool mine_n;
-    pages_at(0, id1);
-    load(0, id1, cur, ks, vs);
-    mine = lane < 2 && id1[lane & 1] >= 0;
-    pages_at(1, id1);
-    for (int u = 0; u < total; ++u) {
-      pages_at(u + 2, id2);
-      if (u + 1 < total) load(u + 1, id1, nxt, ksn, vsn);
-      mine_n = lane < 2 && id1[lane & 1] >= 0;
+    int next[2], later[2];  // page ids two and three positions on
+    const auto step = [&](int u, Held& b) -> bool {
+      pages_at(u + 3, later);
       const int st = u % RS;
-      if (u >= RS && !warp_wait(r_empty + st, ((u / RS) - 1) & 1, p.status, abort)) break;
+      if (u >= RS && !warp_wait(r_empty + st, ((u / RS) - 1) & 1, p.status, abort)) return false;
       int j;
       const bool is_v = what(u, j);
-      const uint32_t dst = sbase + L::RING + st * L::TILE;
+      if (!is_v && lane < 2) {
+        float* sc = scales + (j % NSC) * 24 + cw * 2 + lane;
+        const float k1 = fmaxf(b.ks, 7.8886090522101181e-31f), v1 = fmaxf(b.vs, 7.8886090522101181e-31f);
+        sc[0] = k1;                                   // at least 2^-100: a zero scale stays harmless
+        sc[8] = b.mine ? log2f(v1) : -INFINITY;       // no page: no weight
+        sc[16] = b.mine ? 1.f / v1 : 0.f;
+      }
+      load_scales(next, b);
+      const At at[2] = {page_at(u + 2, next, 0), page_at(u + 2, next, 1)};
+      const uint32_t dst = sbase + L::RING + st * L::TILE + (cw * 32 + t8) * 128 + (((2 * c4) ^ t8) << 4);
 #pragma unroll
       for (int g = 0; g < 4; ++g) {
-        const int tok = cw * 32 + g * 8 + t8;
 #pragma unroll
         for (int sub = 0; sub < NS; ++sub) {
-          const uint4 w = cur[g][sub];
+          const uint4 w = b.reg[g][sub];
           uint32_t x[8];
           q8::decode4_h2<CODE>(w.x, x[0], x[1]);
           q8::decode4_h2<CODE>(w.y, x[2], x[3]);
           q8::decode4_h2<CODE>(w.z, x[4], x[5]);
           q8::decode4_h2<CODE>(w.w, x[6], x[7]);
-          const uint32_t row = dst + sub * SUB + tok * 128;
-          sts128(row + (((2 * c4) ^ t8) << 4), x[0], x[1], x[2], x[3]);
-          sts128(row + (((2 * c4 + 1) ^ t8) << 4), x[4], x[5], x[6], x[7]);
+          sts128(dst + sub * SUB + g * 1024, x[0], x[1], x[2], x[3]);
+          sts128((dst ^ 16) + sub * SUB + g * 1024, x[4], x[5], x[6], x[7]);
+          b.reg[g][sub] = load_one(at[g >> 1], g, sub);
         }
-      }
-      if (!is_v && lane < 2) {
-        float* sc = scales + (j % NSC) * 24 + cw * 2 + lane;
-        const float v1 = fmaxf(vs, 7.8886090522101181e-31f);  // 2^-100: a zero scale stays harmless
-        sc[0] = ks;
-        sc[8] = mine ? log2f(v1) : -INFINITY;                 // no page: no weight
-        sc[16] = mine ? 1.f / v1 : 0.f;
       }
       fence_proxy_async_smem();
       tc::mbar_arrive(r_full + st);
+      next[0] = later[0];
+      next[1] = later[1];
+      return true;
+    };
+    Held even, odd;
+    const auto fill = [&](int u, Held& b) {
+      pages_at(u, next);
+      load_scales(next, b);
+      const At at[2] = {page_at(u, next, 0), page_at(u, next, 1)};
 #pragma unroll
       for (int g = 0; g < 4; ++g)
 #pragma unroll
-        for (int sub = 0; sub < NS; ++sub) cur[g][sub] = nxt[g][sub];
-      ks = ksn;
-      vs = vsn;
-      mine = mine_n;
-      id1[0] = id2[0];
-      id1[1] = id2[1];
+        for (int sub = 0; sub < NS; ++sub) b.reg[g][sub] = load_one(at[g >> 1], g, sub);
+    };
+    fill(0, even);
+    fill(1, odd);
+    pages_at(2, next);
+    for (int u = 0; u < total; u += 2) {  // total is even
+      if (!step(u, even) || !step(u + 1, odd)) break;
     }
   } else {
     // ---- softmax: one thread per query row of tile x -----------------------------------
@@ -350,45 +403,45 @@ __global__ void __launch_bounds__(THREADS, 1) tile_kernel(const Params p) {
     const int row0 = row_a + x * TB, qr = row0 + r;
     const bool valid = nx > 0 && qr < rows;
     const int64_t tok = q_begin + (valid ? qr / p.G : 0), head = h * p.G + (valid ? qr % p.G : 0);
-    float qmul = p.sl2;
+    // a negative softmax scale goes into q's sign: f below stays positive
+    const uint32_t flip = p.sl2 < 0.f ? 0x80008000u : 0u;
+    float qmul = fabsf(p.sl2);
     if (nx > 0) {
       const QT* src = static_cast<const QT*>(p.q) + tok * p.q_stride_t + head * p.q_stride_h;
-      float f = 1.f;
+      uint4 w[D / 8];
+#pragma unroll
+      for (int c = 0; c < D / 8; ++c) w[c] = valid ? reinterpret_cast<const uint4*>(src)[c] : make_uint4(0, 0, 0, 0);
       if (std::is_same<QT, __nv_bfloat16>::value) {
         // bf16 to fp16: a power of two brings the row's largest finite value into [2^13, 2^14)
         uint32_t m = 0;
-        if (valid) {
-#pragma unroll 8
-          for (int c = 0; c < D / 8; ++c) {
-            const uint4 w = reinterpret_cast<const uint4*>(src)[c];
-            const uint32_t u[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const uint32_t lo = (u[i] << 16) & 0x7fffffffu, hi = u[i] & 0x7fff0000u;
-              m = max(m, lo < 0x7f800000u ? lo : 0u);
-              m = max(m, hi < 0x7f800000u ? hi : 0u);
-            }
+        for (int c = 0; c < D / 8; ++c) {
+          const uint32_t* u = reinterpret_cast<const uint32_t*>(&w[c]);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const uint32_t lo = (u[i] << 16) & 0x7fffffffu, hi = u[i] & 0x7fff0000u;
+            m = max(m, lo < 0x7f800000u ? lo : 0u);
+            m = max(m, hi < 0x7f800000u ? hi : 0u);
           }
         }
         const int e = max(static_cast<int>(m >> 23) - 126, -100);
-        f = q8::two_to(14 - e);
-        qmul = q8::two_to(e - 14) * p.sl2;
-      }
-#pragma unroll 8
-      for (int c = 0; c < D / 8; ++c) {
-        uint4 w = make_uint4(0, 0, 0, 0);
-        if (valid) w = reinterpret_cast<const uint4*>(src)[c];
-        if (std::is_same<QT, __nv_bfloat16>::value) {
-          uint32_t* u = reinterpret_cast<uint32_t*>(&w);
+        const float f = q8::two_to(14 - e);
+        qmul *= q8::two_to(e - 14);
+#pragma unroll
+        for (int c = 0; c < D / 8; ++c) {
+          uint32_t* u = reinterpret_cast<uint32_t*>(&w[c]);
 #pragma unroll
           for (int i = 0; i < 4; ++i)
             u[i] = half2_bits(__uint_as_float(u[i] << 16) * f, __uint_as_float(u[i] & 0xffff0000u) * f);
         }
-        sts128(sbase + x * L::TILE + (c >> 3) * SUB + r * 128 + (((c & 7) ^ (r & 7)) << 4), w.x, w.y, w.z, w.w);
       }
-      fence_proxy_async_smem();
-      tc::mbar_arrive(q_full);
+#pragma unroll
+      for (int c = 0; c < D / 8; ++c)
+        sts128(sbase + x * L::TILE + (c >> 3) * SUB + r * 128 + (((c & 7) ^ (r & 7)) << 4), w[c].x ^ flip, w[c].y ^ flip,
+               w[c].z ^ flip, w[c].w ^ flip);
     }
+    fence_proxy_async_smem();
+    tc::mbar_arrive(q_full);
     const int lim = valid ? len - n_tok + qr / p.G + 1 : 0;   // keys that this row sees
     const int lim_all = len - n_tok + row0 / p.G + 1;         // keys that every row of the tile sees
     const uint32_t lane_off = static_cast<uint32_t>(quarter * 32) << 16;
@@ -404,69 +457,78 @@ __global__ void __launch_bounds__(THREADS, 1) tile_kernel(const Params p) {
       tc::tmem_wait_ld();
       tc::fence_before();
       tc::mbar_arrive(s_free);
-      const float* page = scales + (j % NSC) * 24;
-#pragma unroll
-      for (int g = 0; g < 8; ++g) {
-        const poly::f2 f = poly::splat(page[g] * qmul), lv = poly::splat(page[8 + g]);
-#pragma unroll
-        for (int c = 16 * g; c < 16 * g + 16; c += 2)
-          poly::unpack(poly::fma2(poly::pack(sc[c], sc[c + 1]), f, lv), sc[c], sc[c + 1]);
-      }
       if (j * TB + TB > lim_all) {
         const int end = lim - j * TB;
 #pragma unroll
         for (int c = 0; c < TB; ++c) sc[c] = c < end ? sc[c] : -INFINITY;
       }
-      float m8[8];
+      // u = s * f + lv with f > 0: a page's largest u is its largest s's
+      const float4* page = reinterpret_cast<const float4*>(scales + (j % NSC) * 24);
+      float f[8], lv[8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) m8[i] = sc[i];
+      for (int i = 0; i < 2; ++i) {
+        const float4 a = page[i], b = page[2 + i];
+        f[4 * i] = a.x * qmul; f[4 * i + 1] = a.y * qmul; f[4 * i + 2] = a.z * qmul; f[4 * i + 3] = a.w * qmul;
+        lv[4 * i] = b.x; lv[4 * i + 1] = b.y; lv[4 * i + 2] = b.z; lv[4 * i + 3] = b.w;
+      }
+      float mx = -INFINITY;
 #pragma unroll
-      for (int c = 8; c < TB; ++c) m8[c & 7] = fmaxf(m8[c & 7], sc[c]);
-      const float mx = fmaxf(fmaxf(fmaxf(m8[0], m8[1]), fmaxf(m8[2], m8[3])), fmaxf(fmaxf(m8[4], m8[5]), fmaxf(m8[6], m8[7])));
+      for (int g = 0; g < 8; ++g) {
+        const float* v = sc + 16 * g;
+        float m0 = max3(v[0], v[1], v[2]), m1 = max3(v[3], v[4], v[5]);
+        m0 = max3(m0, v[6], v[7]);
+        m1 = max3(m1, v[8], v[9]);
+        m0 = max3(m0, v[10], v[11]);
+        m1 = max3(m1, v[12], v[13]);
+        mx = fmaxf(mx, fmaf(max3(max3(m0, v[14], v[15]), m1, m1), f[g], lv[g]));
+      }
       const float m_new = mx > m_used + SLACK ? mx : m_used;
       const float alpha = m_new == m_used ? 1.f : tc::ex2(m_used - m_new);
-      const poly::f2 neg = poly::splat(m_new == -INFINITY ? 0.f : LIFT - m_new);
+      const float off = m_new == -INFINITY ? 0.f : LIFT - m_new;
+#pragma unroll
+      for (int g = 0; g < 8; ++g) lv[g] += off;
+      if (j >= 1) {  // P V(j - 1) has read P and written O
+        if (!(ok = warp_wait(pv_done + x, (j - 1) & 1, p.status, abort))) break;
+        tc::fence_after();
+        if (__any_sync(FULL_MASK, m_new != m_used)) {
+#pragma unroll 1
+          for (int c = 0; c < D; c += 16) {
+            float o[16];
+            tc::tmem_ld16(to + c, o);
+            tc::tmem_wait_ld();
+#pragma unroll
+            for (int i = 0; i < 16; ++i) o[i] *= alpha;
+            tc::tmem_st16(to + c, o);
+          }
+        }
+      }
       float sum = 0.f;
+      const float* iv = reinterpret_cast<const float*>(page + 4);
 #pragma unroll
       for (int g = 0; g < 8; ++g) {
         float pk[8];
+        const poly::f2 f2 = poly::splat(f[g]), c2 = poly::splat(lv[g]);
         poly::f2 r2[2] = {poly::splat(0.f), poly::splat(0.f)};
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
           float e0, e1;
-          poly::unpack(poly::add2(poly::pack(sc[16 * g + 2 * i], sc[16 * g + 2 * i + 1]), neg), e0, e1);
+          poly::unpack(poly::fma2(poly::pack(sc[16 * g + 2 * i], sc[16 * g + 2 * i + 1]), f2, c2), e0, e1);
           e0 = tc::ex2(e0);
           e1 = tc::ex2(e1);
           r2[i & 1] = poly::add2(r2[i & 1], poly::pack(e0, e1));
           pk[i] = __uint_as_float(half2_bits(e0, e1));
         }
-        float r4[4];
-        poly::unpack(r2[0], r4[0], r4[1]);
-        poly::unpack(r2[1], r4[2], r4[3]);
-        sum = fmaf((r4[0] + r4[1]) + (r4[2] + r4[3]), page[16 + g], sum);
-        if (g == 0 && j >= 1) {
-          if (!(ok = warp_wait(pv_done + x, (j - 1) & 1, p.status, abort))) break;
-          tc::fence_after();
-        }
         tc::tmem_st8(tp + 8 * g, pk);
-      }
-      if (!ok) break;
-      l = fmaf(l, alpha, sum);
-      if (j >= 1 && __any_sync(FULL_MASK, m_new != m_used)) {
-        const float f = m_new != m_used ? alpha : 1.f;
-#pragma unroll 1
-        for (int c = 0; c < D; c += 16) {
-          float o[16];
-          tc::tmem_ld16(to + c, o);
-          tc::tmem_wait_ld();
-#pragma unroll
-          for (int i = 0; i < 16; ++i) o[i] *= f;
-          tc::tmem_st16(to + c, o);
+        if (g == 3 || g == 7) {
+          tc::tmem_wait_st();
+          tc::fence_before();
+          tc::mbar_arrive(p_full + 2 * x + (g >> 2));
         }
+        float r4[4];
+        poly::unpack(poly::add2(r2[0], r2[1]), r4[0], r4[1]);
+        sum = fmaf(r4[0] + r4[1], iv[g], sum);
       }
-      tc::tmem_wait_st();
-      tc::fence_before();
-      tc::mbar_arrive(p_full + x);
+      l = fmaf(l, alpha, sum);
       m_used = m_new;
     }
     if (nx > 0 && ok) ok = warp_wait(pv_done + x, (nx - 1) & 1, p.status, abort);
