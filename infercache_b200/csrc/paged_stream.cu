@@ -45,15 +45,16 @@ namespace ic {
 namespace paged {
 namespace {
 
+constexpr int SMS = 148;
 constexpr int NW = 8;                 // warps per CTA
+constexpr float TINY = 7.8886090522101181e-31f;  // 2^-100
 constexpr float SLACK = 8.f;          // u may pass M by this much
 constexpr float LIFT = 7.f;           // P' = 2^(u - M + LIFT): at most 2^15
 
-// CTAs per SM (two where 128 registers a thread hold q and O without spills)
-// and ring stages per warp: 96 KB of pages in flight per CTA, twice that where
-// it has the SM to itself.
+// CTAs per SM: two where 128 registers a thread hold q and O without spills.
+// Ring stages per warp: what their shared memory leaves beside the merge rows.
 __host__ __device__ constexpr int ctas_per_sm(int D, int NG) { return D * NG > 128 ? 1 : 2; }
-__host__ __device__ constexpr int stages(int D, int NG) { return (ctas_per_sm(D, NG) == 1 ? 192 : 96) * 1024 / (NW * 32 * D); }
+__host__ __device__ constexpr int stages(int D, int NG) { return D == 256 ? 2 : D == 64 ? 5 : NG == 2 ? 5 : 2; }
 
 struct Task {  // the group that continues past a CTA's share, when it begins there
   int32_t valid, s, h, tile, last_cta, first_slot;
@@ -66,9 +67,8 @@ struct Layout {
   static constexpr int RING = NW * ST * 2 * PAGE_B;
   static constexpr int ROWS = 8 * NG;
   static constexpr int PITCH = D + 4;                        // floats per row of a warp's O
-  static constexpr int MERGE = NW * ROWS * PITCH * 4;        // aliases the ring
-  static constexpr int BUF = RING > MERGE ? RING : MERGE;
-  static constexpr int BARS = BUF;
+  static constexpr int MERGE = RING;                         // 8 rows of every warp's O
+  static constexpr int BARS = MERGE + NW * 8 * PITCH * 4;
   static constexpr int STAT = BARS + NW * ST * 8;            // M, l per warp and row
   static constexpr int SCAN = STAT + NW * ROWS * 8;
   static constexpr int PREFIX = SCAN + 64;
@@ -126,6 +126,19 @@ __device__ __forceinline__ uint32_t max_magnitude(uint32_t m, const uint4& v) { 
   return m;
 }
 
+// Four finished elements x / l; no key at all gives zeros, NaN stays NaN.
+template <typename QT>
+__device__ __forceinline__ void store_row(QT* dst, const float4& x, float l) {
+  const float inv = l > 0.f ? 1.f / l : l == l ? 0.f : l;
+  const auto pair = [&](float a, float b) {
+    return static_cast<uint32_t>(Mma<QT>::bits(a * inv)) | (static_cast<uint32_t>(Mma<QT>::bits(b * inv)) << 16);
+  };
+  *reinterpret_cast<uint2*>(dst) = make_uint2(pair(x.x, x.y), pair(x.z, x.w));
+}
+__device__ __forceinline__ float lse_of(float m, float l) {
+  return l > 0.f ? (m - LIFT + log2f(l)) * LN2 : l == l ? -INFINITY : l;
+}
+
 template <typename QT, int D, int CODE, int NG>
 __global__ void __launch_bounds__(NW * 32, ctas_per_sm(D, NG))
     stream_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv, const Params p) {
@@ -150,17 +163,30 @@ __global__ void __launch_bounds__(NW * 32, ctas_per_sm(D, NG))
   grid_launch_dependents();
 
   // ---- the line of all groups' pages: prefix sums over the sessions -----------
-  {
+  // Up to 32 sessions live in the lanes of every warp; more, in shared memory.
+  const bool lanes = p.S <= 32;
+  int l_begin = 0, l_tok = 0, l_len = 0, l_upto = 0, total;
+  const auto units_of = [&](int x, int& begin, int& tok, int& len) {
+    tok = query_tokens(p, x, begin);
+    len = held_tokens(p, x);
+    const int rows = tok * p.G;
+    return rows <= p.few_rows ? (rows + ROWS - 1) / ROWS * p.H * max(1, (len + q8::PAGE - 1) / q8::PAGE) : 0;
+  };
+  if (lanes) {
+    if (lane < p.S) l_upto = units_of(lane, l_begin, l_tok, l_len);
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int u = __shfl_up_sync(FULL_MASK, l_upto, o);
+      if (lane >= o) l_upto += u;
+    }
+    total = __shfl_sync(FULL_MASK, l_upto, 31);
+    __syncthreads();  // the barriers are initialised
+  } else {
     int carry = 0;
     for (int s0 = 0; s0 < p.S; s0 += NW * 32) {
       const int s = s0 + tid;
-      int w = 0;
-      if (s < p.S) {
-        int begin;
-        const int rows = query_tokens(p, s, begin) * p.G;
-        const int pages = max(1, (held_tokens(p, s) + q8::PAGE - 1) / q8::PAGE);
-        if (rows <= p.few_rows) w = (rows + ROWS - 1) / ROWS * p.H * pages;
-      }
+      int w = 0, x, y, z;
+      if (s < p.S) w = units_of(s, x, y, z);
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
         const int u = __shfl_up_sync(FULL_MASK, w, o);
@@ -177,8 +203,8 @@ __global__ void __launch_bounds__(NW * 32, ctas_per_sm(D, NG))
       if (s < p.S) prefix[s + 1] = before + w;
       __syncthreads();
     }
+    total = prefix[p.S];
   }
-  const int total = prefix[p.S];
   const int share = max((total + static_cast<int>(gridDim.x) - 1) / static_cast<int>(gridDim.x), p.min_share);
   const int cta = blockIdx.x;
   const int64_t pos0 = static_cast<int64_t>(cta) * share;
@@ -193,73 +219,97 @@ __global__ void __launch_bounds__(NW * 32, ctas_per_sm(D, NG))
   uint64_t* wbar = bars + warp * ST;
   uint32_t phases = 0;   // bit i: parity of the next wait on stage i
   bool dead = false;     // a wait gave up: nothing more is loaded
-  int s = 0;
-  int pos = static_cast<int>(pos0);
-  while (pos < end) {
-    // ---- the segment: session s, KV head h, row tile, pages p0 .. p1 ------------
-    {
-      int lo = s, hi = p.S;  // the last session whose first unit is <= pos
+  int st = 0;            // stage of the next page to be consumed
+
+  // A segment: session s, KV head h, row tile, pages p0 .. p1 of the group; this
+  // warp's are p0 + warp + NW * i, i < mine.
+  struct Seg {
+    int s, h, q_begin, n_tok, len, row0, pages, p0, p1, mine;
+  };
+  const auto find = [&](int pos, int from) {
+    Seg g;
+    int before;
+    if (lanes) {
+      g.s = __popc(__ballot_sync(FULL_MASK, l_upto <= pos));
+      before = __shfl_sync(FULL_MASK, l_upto, max(g.s - 1, 0));
+      if (g.s == 0) before = 0;
+      g.q_begin = __shfl_sync(FULL_MASK, l_begin, g.s);
+      g.n_tok = __shfl_sync(FULL_MASK, l_tok, g.s);
+      g.len = __shfl_sync(FULL_MASK, l_len, g.s);
+    } else {
+      int lo = from, hi = p.S;  // the last session whose first unit is <= pos
       while (hi - lo > 1) {
         const int mid = (lo + hi) >> 1;
         if (prefix[mid] <= pos) lo = mid; else hi = mid;
       }
-      s = lo;
+      g.s = lo;
+      before = prefix[lo];
+      g.n_tok = query_tokens(p, lo, g.q_begin);
+      g.len = held_tokens(p, lo);
     }
-    int q_begin;
-    const int n_tok = query_tokens(p, s, q_begin), rows = n_tok * p.G, len = held_tokens(p, s);
-    const int pages = max(1, (len + q8::PAGE - 1) / q8::PAGE), tiles = (rows + ROWS - 1) / ROWS;
-    const int gi = (pos - prefix[s]) / pages, p0 = (pos - prefix[s]) % pages;
-    const int p1 = min(pages, p0 + (end - pos));
-    const int h = gi / tiles, row0 = gi % tiles * ROWS;
-    const int group_begin = pos - p0, group_end = group_begin + pages;
-    const int mine = max(0, (p1 - p0 - warp + NW - 1) / NW);   // this warp's pages: p0 + warp + NW * i
-    const int32_t* trow = p.table + static_cast<int64_t>(s) * p.width + p0 + warp;
-    const float* ksh = p.k_scale + static_cast<int64_t>(h) * p.n_pages;
-    const float* vsh = p.v_scale + static_cast<int64_t>(h) * p.n_pages;
-
-    // lane j holds page 32 * batch + j of this warp: id, K scale, log2 and
-    // reciprocal of the V scale (at least 2^-100, so a zero scale stays harmless);
-    // the next batch beside it
-    int id_c, id_n = -1;
-    float ks_c, lv_c, iv_c, ks_n = 0.f, lv_n = 0.f, iv_n = 1.f;
-    const auto fetch = [&](int base, int& id, float& ks, float& lv, float& iv) {
-      id = -1;
-      ks = 0.f;
-      float vs = 1.f;
-      const int i = base + lane;
-      if (i < mine && (p0 + warp + NW * i) * q8::PAGE < len) {
-        const int x = trow[NW * i];
-        if (static_cast<unsigned>(x) < static_cast<unsigned>(p.n_pages)) {
-          id = x;
-          ks = ksh[x];
-          vs = fmaxf(vsh[x], 7.8886090522101181e-31f);
-        } else if (p.status) {
-          atomicOr(p.status, IC_DEVFLAG_BAD_ROW);
-        }
+    g.pages = max(1, (g.len + q8::PAGE - 1) / q8::PAGE);
+    const int tiles = (g.n_tok * p.G + ROWS - 1) / ROWS, at = pos - before, gi = at / g.pages;
+    g.p0 = at - gi * g.pages;
+    g.p1 = min(g.pages, g.p0 + (end - pos));
+    g.h = gi / tiles;
+    g.row0 = (gi - g.h * tiles) * ROWS;
+    g.mine = max(0, (g.p1 - g.p0 - warp + NW - 1) / NW);
+    return g;
+  };
+  // Lane j holds page base + j of this warp: its id, then its K scale and the
+  // logarithm and reciprocal of its V scale (both at least 2^-100, so a zero
+  // scale stays harmless).
+  const auto fetch_id = [&](const Seg& g, int base) {
+    const int i = base + lane, pg = g.p0 + warp + NW * i;
+    int id = -1;
+    if (i < g.mine && pg * q8::PAGE < g.len) {
+      id = p.table[static_cast<int64_t>(g.s) * p.width + pg];
+      if (static_cast<unsigned>(id) >= static_cast<unsigned>(p.n_pages)) {
+        id = -1;
+        if (p.status) atomicOr(p.status, IC_DEVFLAG_BAD_ROW);
       }
-      lv = log2f(vs);
-      iv = 1.f / vs;
-    };
-    const auto issue = [&](int i, int page) {
-      const int st = i % ST;
-      if (lane == 0 && page >= 0 && !dead) {
-        unsigned char* dst = smem + warp * (ST * 2 * L::PAGE_B) + st * 2 * L::PAGE_B;
-        mbar_arrive_expect_tx(wbar + st, 2 * L::PAGE_B);
-        const int y = D == 64 ? page * 8 : page * 16;
+    }
+    return id;
+  };
+  const auto fetch_scales = [&](const Seg& g, int id, float& ks, float& vs) {
+    ks = vs = 1.f;
+    if (id >= 0) {
+      ks = p.k_scale[static_cast<int64_t>(g.h) * p.n_pages + id];
+      vs = p.v_scale[static_cast<int64_t>(g.h) * p.n_pages + id];
+    }
+  };
+  const auto issue = [&](const Seg& g, int stage, int page) {
+    if (lane == 0 && page >= 0 && !dead) {
+      unsigned char* dst = smem + warp * (ST * 2 * L::PAGE_B) + stage * 2 * L::PAGE_B;
+      mbar_arrive_expect_tx(wbar + stage, 2 * L::PAGE_B);
+      const int y = D == 64 ? page * 8 : page * 16;
 #pragma unroll
-        for (int x = 0; x < (D == 256 ? 2 : 1); ++x) {
-          tc::tma_load_3d(dst + x * 2048, &mk, x * 128, y, h, wbar + st);
-          tc::tma_load_3d(dst + L::PAGE_B + x * 2048, &mv, x * 128, y, h, wbar + st);
-        }
+      for (int x = 0; x < (D == 256 ? 2 : 1); ++x) {
+        tc::tma_load_3d(dst + x * 2048, &mk, x * 128, y, g.h, wbar + stage);
+        tc::tma_load_3d(dst + L::PAGE_B + x * 2048, &mv, x * 128, y, g.h, wbar + stage);
       }
-    };
-    fetch(0, id_c, ks_c, lv_c, iv_c);
+    }
+  };
+  const auto wrap = [](int x) { return x >= ST ? x - ST : x; };
+  // The first ST pages of a segment; the ring is empty when this is called.
+  const auto begin_pages = [&](const Seg& g, int id) {
 #pragma unroll
     for (int i = 0; i < ST; ++i) {
-      const int page = __shfl_sync(FULL_MASK, id_c, i);
-      if (i < mine) issue(i, page);
+      const int page = __shfl_sync(FULL_MASK, id, i);
+      if (i < g.mine) issue(g, wrap(st + i), page);
     }
-    if (mine > 32) fetch(32, id_n, ks_n, lv_n, iv_n);
+  };
+
+  int pos = static_cast<int>(pos0);
+  Seg seg = find(pos, 0);
+  int id_c = fetch_id(seg, 0);
+  begin_pages(seg, id_c);
+  for (;;) {
+    const int s = seg.s, h = seg.h, len = seg.len, rows = seg.n_tok * p.G, row0 = seg.row0, mine = seg.mine;
+    float ks_c, vs_c, ks_n = 1.f, vs_n = 1.f;
+    int id_n = -1;
+    fetch_scales(seg, id_c, ks_c, vs_c);
+    if (mine > 32) id_n = fetch_id(seg, 32);
 
     // ---- q as the B operand; head rows past the session's are zero ---------------
     uint32_t qb[NG][NC * 4][2];
@@ -270,7 +320,7 @@ __global__ void __launch_bounds__(NW * 32, ctas_per_sm(D, NG))
       const int r = row0 + nt * 8 + g;
       const bool ok = r < rows;
       const QT* src = static_cast<const QT*>(p.q);
-      if (ok) src += (q_begin + r / p.G) * p.q_stride_t + (h * p.G + r % p.G) * p.q_stride_h;
+      if (ok) src += (seg.q_begin + r / p.G) * p.q_stride_t + (h * p.G + r % p.G) * p.q_stride_h;
       uint4 va[NC], vb[NC];
 #pragma unroll
       for (int c = 0; c < NC; ++c) {
@@ -309,10 +359,13 @@ __global__ void __launch_bounds__(NW * 32, ctas_per_sm(D, NG))
       for (int i = 0; i < 2; ++i) {
         qmul[nt][i] = __shfl_sync(FULL_MASK, back, (2 * tq + i) * 4) * p.sl2;
         const int ri = row0 + nt * 8 + 2 * tq + i;
-        lim[nt][i] = ri < rows ? len - n_tok + ri / p.G + 1 : 0;
+        lim[nt][i] = ri < rows ? len - seg.n_tok + ri / p.G + 1 : 0;
       }
     }
-    const int lim_all = len - n_tok + row0 / p.G + 1;  // keys that every row of the tile sees
+    const int lim_all = len - seg.n_tok + row0 / p.G + 1;  // keys that every row of the tile sees
+    ks_c = fmaxf(ks_c, TINY);
+    vs_c = fmaxf(vs_c, TINY);
+    float lv_c = log2f(vs_c), iv_c = 1.f / vs_c;
 
     float M[NG][2], l[NG][2], o[NG][MT][4];
 #pragma unroll
@@ -324,18 +377,25 @@ __global__ void __launch_bounds__(NW * 32, ctas_per_sm(D, NG))
     }
 
     // ---- stream ---------------------------------------------------------------------
+#pragma unroll 1
     for (int i = 0; i < mine; ++i) {
-      if (i > 0 && (i & 31) == 0) {
-        id_c = id_n;
-        ks_c = ks_n;
-        lv_c = lv_n;
-        iv_c = iv_n;
-        if (i + 32 < mine) fetch(i + 32, id_n, ks_n, lv_n, iv_n);
+      if ((i & 31) == 0) {
+        if (i > 0) {
+          id_c = id_n;
+          ks_c = fmaxf(ks_n, TINY);
+          vs_c = fmaxf(vs_n, TINY);
+          lv_c = log2f(vs_c);
+          iv_c = 1.f / vs_c;
+          id_n = i + 32 < mine ? fetch_id(seg, i + 32) : -1;
+        }
+        fetch_scales(seg, id_n, ks_n, vs_n);
       }
       const int page = __shfl_sync(FULL_MASK, id_c, i & 31);
       const float ks = __shfl_sync(FULL_MASK, ks_c, i & 31);
       const float lv = __shfl_sync(FULL_MASK, lv_c, i & 31), inv_vs = __shfl_sync(FULL_MASK, iv_c, i & 31);
-      const int st = i % ST;
+      const int nx = i + ST;  // the page that takes this one's stage
+      const int next_c = __shfl_sync(FULL_MASK, id_c, nx & 31), next_n = __shfl_sync(FULL_MASK, id_n, nx & 31);
+      const int next = nx < mine ? ((nx >> 5) == (i >> 5) ? next_c : next_n) : -1;
       if (page >= 0 && !dead) {
         const bool ok = mbar_wait_bounded(wbar + st, (phases >> st) & 1, p.status);
         dead = !__all_sync(FULL_MASK, ok);
@@ -343,10 +403,13 @@ __global__ void __launch_bounds__(NW * 32, ctas_per_sm(D, NG))
       }
       if (page >= 0 && !dead) {
         const uint32_t kp = ring + st * 2 * L::PAGE_B, vp = kp + L::PAGE_B;
-        const int tok0 = (p0 + warp + NW * i) * q8::PAGE;
-        float acc[NG][4];
+        const int tok0 = (seg.p0 + warp + NW * i) * q8::PAGE;
+        // two chains of products where one row tile would leave a single long one
+        float acc[NG][4], odd[NG == 1 ? 1 : NG][4];
 #pragma unroll
-        for (int nt = 0; nt < NG; ++nt) acc[nt][0] = acc[nt][1] = acc[nt][2] = acc[nt][3] = 0.f;
+        for (int nt = 0; nt < NG; ++nt)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc[nt][e] = odd[nt][e] = 0.f;
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
           const int chunk = D == 64 ? tq : (c >> 1) * 8 + 2 * tq + (c & 1);
@@ -359,9 +422,39 @@ __global__ void __launch_bounds__(NW * 32, ctas_per_sm(D, NG))
             q8::decode4_h2<CODE>(w1[j], a1, a3);
 #pragma unroll
             for (int nt = 0; nt < NG; ++nt)
-              Mma<__half>::run(acc[nt], a0, a1, a2, a3, qb[nt][c * 4 + j][0], qb[nt][c * 4 + j][1]);
+              Mma<__half>::run(NG == 1 && (j & 1) ? odd[nt] : acc[nt], a0, a1, a2, a3, qb[nt][c * 4 + j][0], qb[nt][c * 4 + j][1]);
           }
         }
+        if (NG == 1) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc[0][e] += odd[0][e];
+        }
+        // V: tokens 2 tq, 2 tq + 1, 2 tq + 8, 2 tq + 9; this lane's D / 8 dims from D / 8 * g
+        uint32_t t[4][W4];
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          const int tok = 2 * tq + (x & 1) + (x >> 1) * 8;
+          if (D == 64) {
+            const uint2 v = lds64(vp + page_off<D>(tok, g >> 1) + (g & 1) * 8);
+            t[x][0] = v.x;
+            t[x][1] = v.y;
+          } else {
+#pragma unroll
+            for (int c = 0; c < W4 / 4; ++c) {
+              const uint4 v = lds128(vp + page_off<D>(tok, g * (W4 / 4) + c));
+              t[x][4 * c] = v.x;
+              t[x][4 * c + 1] = v.y;
+              t[x][4 * c + 2] = v.z;
+              t[x][4 * c + 3] = v.w;
+            }
+          }
+          if (tok0 + q8::PAGE > len && tok0 + tok >= len) {  // nothing of an earlier owner's rows
+#pragma unroll
+            for (int c = 0; c < W4; ++c) t[x][c] = 0;
+          }
+        }
+        __syncwarp();  // the page is in registers: its stage takes the next one
+        issue(seg, st, next);
         const bool edge = tok0 + q8::PAGE > lim_all;
         bool over = false;
 #pragma unroll
@@ -408,30 +501,6 @@ __global__ void __launch_bounds__(NW * 32, ctas_per_sm(D, NG))
           pb[nt][0] = transpose8(half2_bits(pr[0], pr[1]));
           pb[nt][1] = transpose8(half2_bits(pr[2], pr[3]));
         }
-        // V: tokens 2 tq, 2 tq + 1, 2 tq + 8, 2 tq + 9; this lane's D / 8 dims from D / 8 * g
-        uint32_t t[4][W4];
-#pragma unroll
-        for (int x = 0; x < 4; ++x) {
-          const int tok = 2 * tq + (x & 1) + (x >> 1) * 8;
-          if (D == 64) {
-            const uint2 v = lds64(vp + page_off<D>(tok, g >> 1) + (g & 1) * 8);
-            t[x][0] = v.x;
-            t[x][1] = v.y;
-          } else {
-#pragma unroll
-            for (int c = 0; c < W4 / 4; ++c) {
-              const uint4 v = lds128(vp + page_off<D>(tok, g * (W4 / 4) + c));
-              t[x][4 * c] = v.x;
-              t[x][4 * c + 1] = v.y;
-              t[x][4 * c + 2] = v.z;
-              t[x][4 * c + 3] = v.w;
-            }
-          }
-          if (tok0 + q8::PAGE > len && tok0 + tok >= len) {  // nothing of an earlier owner's rows
-#pragma unroll
-            for (int c = 0; c < W4; ++c) t[x][c] = 0;
-          }
-        }
 #pragma unroll
         for (int c = 0; c < W4; ++c) {
 #pragma unroll
@@ -444,16 +513,24 @@ __global__ void __launch_bounds__(NW * 32, ctas_per_sm(D, NG))
               Mma<__half>::run(o[nt][2 * c + half], a0, a1, a2, a3, pb[nt][0], pb[nt][1]);
           }
         }
+      } else {
+        issue(seg, st, next);
       }
-      __syncwarp();
-      {
-        const int nx = i + ST;
-        const int from_c = __shfl_sync(FULL_MASK, id_c, nx & 31), from_n = __shfl_sync(FULL_MASK, id_n, nx & 31);
-        if (nx < mine) issue(nx, (nx >> 5) == (i >> 5) ? from_c : from_n);
-      }
+      st = wrap(st + 1);
     }
     if (dead) {  // copies in flight land before their buffers are given up (short waits)
-      for (int st = 0; st < ST; ++st) mbar_wait_bounded(wbar + st, (phases >> st) & 1, nullptr, 200000000ull);
+      for (int x = 0; x < ST; ++x) mbar_wait_bounded(wbar + x, (phases >> x) & 1, nullptr, 200000000ull);
+    }
+
+    // ---- the next segment's first pages are on their way while this one is joined ------
+    const int next_pos = pos + seg.p1 - seg.p0;
+    const bool more = next_pos < end;
+    Seg nseg;
+    int nid = -1;
+    if (more) {
+      nseg = find(next_pos, s);
+      nid = fetch_id(nseg, 0);
+      begin_pages(nseg, nid);
     }
 #pragma unroll
     for (int nt = 0; nt < NG; ++nt)
@@ -462,83 +539,80 @@ __global__ void __launch_bounds__(NW * 32, ctas_per_sm(D, NG))
 #pragma unroll
         for (int x = 4; x < 32; x <<= 1) l[nt][e] += __shfl_xor_sync(FULL_MASK, l[nt][e], x);
 
-    // ---- join the warps ---------------------------------------------------------------
-    __syncthreads();  // every warp is done with its ring, which the O rows alias
-    float* wo = reinterpret_cast<float*>(smem);
+    // ---- join the warps, 8 rows at a time ----------------------------------------------
+    float* wo = reinterpret_cast<float*>(smem + L::MERGE);
+    const bool whole = seg.p0 == 0 && seg.p1 == seg.pages;
+    const int slot = 2 * cta + (pos == pos0 ? 0 : 1);
 #pragma unroll
     for (int nt = 0; nt < NG; ++nt) {
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        const int row = nt * 8 + 2 * tq + e;
-        float* dst = wo + (warp * ROWS + row) * L::PITCH + (D / 8) * g;
+        const int row = 2 * tq + e;
+        float* dst = wo + (warp * 8 + row) * L::PITCH + (D / 8) * g;
         // elements 2 mt + {0, 1} of this lane's dims are o[mt][e], o[mt][e + 2]
 #pragma unroll
         for (int c = 0; c < MT / 2; ++c)
           reinterpret_cast<float4*>(dst)[c] =
               make_float4(o[nt][2 * c][e], o[nt][2 * c][e + 2], o[nt][2 * c + 1][e], o[nt][2 * c + 1][e + 2]);
-        if (g == 0) {
-          stat[(warp * ROWS + row) * 2] = M[nt][e];
-          stat[(warp * ROWS + row) * 2 + 1] = l[nt][e];
+        if (g == 0) *reinterpret_cast<float2*>(stat + (warp * 8 + row) * 2) = make_float2(M[nt][e], l[nt][e]);
+      }
+      __syncthreads();
+      for (int e = tid; e < 8 * (D / 4); e += NW * 32) {
+        const int row = e / (D / 4), d0 = e % (D / 4) * 4, r = row0 + nt * 8 + row;
+        float2 ml[NW];
+        float m = -INFINITY, lsum = 0.f;
+#pragma unroll
+        for (int w = 0; w < NW; ++w) {
+          ml[w] = *reinterpret_cast<const float2*>(stat + (w * 8 + row) * 2);
+          m = fmaxf(m, ml[w].x);
+        }
+        float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int w = 0; w < NW; ++w) {
+          const float f = ml[w].x == -INFINITY ? 0.f : tc::ex2(ml[w].x - m);
+          lsum = fmaf(ml[w].y, f, lsum);
+          const float4 u = *reinterpret_cast<const float4*>(wo + (w * 8 + row) * L::PITCH + d0);
+          x.x = fmaf(u.x, f, x.x); x.y = fmaf(u.y, f, x.y); x.z = fmaf(u.z, f, x.z); x.w = fmaf(u.w, f, x.w);
+        }
+        const size_t prow = static_cast<size_t>(slot) * ROWS + nt * 8 + row;
+        if (!whole) {
+          *reinterpret_cast<float4*>(part + prow * D + d0) = x;
+          if (d0 == 0) *reinterpret_cast<float2*>(part_stat + prow * 2) = make_float2(m, lsum);
+        } else if (r < rows) {
+          const int64_t orow = static_cast<int64_t>(seg.q_begin + r / p.G) * p.Hq + h * p.G + r % p.G;
+          store_row<QT>(static_cast<QT*>(p.out) + orow * D + d0, x, lsum);
+          if (d0 == 0 && p.lse) p.lse[orow] = lse_of(m, lsum);
         }
       }
+      __syncthreads();
     }
-    __syncthreads();
-    const bool whole = p0 == 0 && p1 == pages;
-    const int slot = 2 * cta + (pos == pos0 ? 0 : 1);
-    for (int e = tid; e < ROWS * (D / 4); e += NW * 32) {
-      const int row = e / (D / 4), d0 = e % (D / 4) * 4, r = row0 + row;
-      float m = -INFINITY, lsum = 0.f;
-#pragma unroll
-      for (int w = 0; w < NW; ++w) m = fmaxf(m, stat[(w * ROWS + row) * 2]);
-      float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-      for (int w = 0; w < NW; ++w) {
-        const float mw = stat[(w * ROWS + row) * 2];
-        const float f = mw == -INFINITY ? 0.f : tc::ex2(mw - m);
-        lsum = fmaf(stat[(w * ROWS + row) * 2 + 1], f, lsum);
-        const float4 u = *reinterpret_cast<const float4*>(wo + (w * ROWS + row) * L::PITCH + d0);
-        x.x = fmaf(u.x, f, x.x); x.y = fmaf(u.y, f, x.y); x.z = fmaf(u.z, f, x.z); x.w = fmaf(u.w, f, x.w);
-      }
-      if (!whole) {
-        *reinterpret_cast<float4*>(part + (static_cast<size_t>(slot) * ROWS + row) * D + d0) = x;
-        if (d0 == 0) {
-          part_stat[(static_cast<size_t>(slot) * ROWS + row) * 2] = m;
-          part_stat[(static_cast<size_t>(slot) * ROWS + row) * 2 + 1] = lsum;
-        }
-      } else if (r < rows) {
-        const float inv = lsum > 0.f ? 1.f / lsum : lsum == lsum ? 0.f : lsum;  // NaN stays NaN
-        const int64_t orow = static_cast<int64_t>(q_begin + r / p.G) * p.Hq + h * p.G + r % p.G;
-        QT* dst = static_cast<QT*>(p.out) + orow * D + d0;
-        const uint32_t lo = static_cast<uint32_t>(Mma<QT>::bits(x.x * inv)) | (static_cast<uint32_t>(Mma<QT>::bits(x.y * inv)) << 16);
-        const uint32_t hi = static_cast<uint32_t>(Mma<QT>::bits(x.z * inv)) | (static_cast<uint32_t>(Mma<QT>::bits(x.w * inv)) << 16);
-        *reinterpret_cast<uint2*>(dst) = make_uint2(lo, hi);
-        if (d0 == 0 && p.lse) p.lse[orow] = lsum > 0.f ? (m - LIFT + log2f(lsum)) * LN2 : lsum == lsum ? -INFINITY : lsum;
-      }
-    }
-    if (tid == 0 && !whole && p1 < pages && group_begin >= pos0) {  // this CTA holds the group's first page, not its last
+    if (tid == 0 && seg.p0 == 0 && seg.p1 < seg.pages) {  // this CTA holds the group's first page, not its last
       Task t;
       t.valid = 1;
       t.s = s;
       t.h = h;
       t.tile = row0 / ROWS;
-      t.last_cta = (group_end - 1) / share;
+      t.last_cta = (pos + seg.pages - 1) / share;
       t.first_slot = slot;
       tasks[cta] = t;
     }
-    pos += p1 - p0;
-    fence_proxy_async_smem();  // the O rows were written through the generic proxy; copies follow
-    __syncthreads();
+    if (!more) break;
+    pos = next_pos;
+    seg = nseg;
+    id_c = nid;
   }
 }
 
 // Joins the partials of the groups that lie in several shares: one CTA per
-// (CTA where such a group begins, row).  Eight subgroups of lanes take every
-// eighth partial each; their sums are joined in order.
+// (CTA where such a group begins, row).  The weights of all partials come first
+// (a thread each), then eight subgroups of lanes add every eighth partial and
+// their sums are joined in order.
 template <typename QT, int D, int NG>
 __global__ void __launch_bounds__(8 * (D / 4)) join_kernel(const Params p, int ctas) {
-  constexpr int ROWS = 8 * NG, LN = D / 4;
+  constexpr int ROWS = 8 * NG, LN = D / 4, NT = 8 * LN, MAXP = 2 * SMS;
+  __shared__ float weight[MAXP];
   __shared__ float4 sx[8][LN];
-  __shared__ float sl[8];
+  __shared__ float red[2][NT / 32];
   grid_dependency_wait();
   grid_launch_dependents();
   const float* part = p.ws;
@@ -550,51 +624,59 @@ __global__ void __launch_bounds__(8 * (D / 4)) join_kernel(const Params p, int c
   const int rows = query_tokens(p, t.s, q_begin) * p.G;
   const int row = blockIdx.y, r = t.tile * ROWS + row;
   if (r >= rows) return;
-  const int sub = threadIdx.x / LN, ln = threadIdx.x % LN;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, sub = tid / LN, ln = tid % LN;
   const int n = t.last_cta - static_cast<int>(blockIdx.x) + 1;
   // partial i: the first share's, then slot 0 of each later one
   const auto at = [&](int i) {
     return (static_cast<size_t>(i == 0 ? t.first_slot : 2 * (blockIdx.x + i)) * ROWS + row);
   };
-  float m = -INFINITY;
-  for (int i = sub; i < n; i += 8) m = fmaxf(m, part_stat[at(i) * 2]);
-  if (ln == 0) sl[sub] = m;
+  constexpr int PER = (MAXP + NT - 1) / NT;
+  float2 ml[PER];
+  float m = -INFINITY, lsum = 0.f;
+#pragma unroll
+  for (int k = 0; k < PER; ++k) {
+    const int i = tid + k * NT;
+    ml[k] = make_float2(-INFINITY, 0.f);
+    if (i < n) ml[k] = *reinterpret_cast<const float2*>(part_stat + at(i) * 2);
+    m = fmaxf(m, ml[k].x);
+  }
+  m = warp_max(m);
+  if (lane == 0) red[0][warp] = m;
   __syncthreads();
 #pragma unroll
-  for (int i = 0; i < 8; ++i) m = fmaxf(m, sl[i]);
+  for (int i = 0; i < NT / 32; ++i) m = fmaxf(m, red[0][i]);
+#pragma unroll
+  for (int k = 0; k < PER; ++k) {
+    const int i = tid + k * NT;
+    const float f = ml[k].x == -INFINITY ? 0.f : tc::ex2(ml[k].x - m);
+    if (i < n) weight[i] = f;
+    lsum = fmaf(ml[k].y, f, lsum);
+  }
+  lsum = warp_sum(lsum);
+  if (lane == 0) red[1][warp] = lsum;
   __syncthreads();
   float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-  float lsum = 0.f;
-#pragma unroll 4
+#pragma unroll 8
   for (int i = sub; i < n; i += 8) {
-    const float mi = part_stat[at(i) * 2], li = part_stat[at(i) * 2 + 1];
     const float4 u = *reinterpret_cast<const float4*>(part + at(i) * D + 4 * ln);
-    const float f = mi == -INFINITY ? 0.f : tc::ex2(mi - m);
-    lsum = fmaf(li, f, lsum);
+    const float f = weight[i];
     x.x = fmaf(u.x, f, x.x); x.y = fmaf(u.y, f, x.y); x.z = fmaf(u.z, f, x.z); x.w = fmaf(u.w, f, x.w);
   }
   sx[sub][ln] = x;
-  if (ln == 0) sl[sub] = lsum;
   __syncthreads();
   if (sub != 0) return;
   lsum = 0.f;
-  x = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
+  for (int i = 0; i < NT / 32; ++i) lsum += red[1][i];
+#pragma unroll
+  for (int i = 1; i < 8; ++i) {
     const float4 u = sx[i][ln];
     x.x += u.x; x.y += u.y; x.z += u.z; x.w += u.w;
-    lsum += sl[i];
   }
-  const float inv = lsum > 0.f ? 1.f / lsum : lsum == lsum ? 0.f : lsum;
   const int64_t orow = static_cast<int64_t>(q_begin + r / p.G) * p.Hq + t.h * p.G + r % p.G;
-  QT* dst = static_cast<QT*>(p.out) + orow * D + 4 * ln;
-  const uint32_t lo = static_cast<uint32_t>(Mma<QT>::bits(x.x * inv)) | (static_cast<uint32_t>(Mma<QT>::bits(x.y * inv)) << 16);
-  const uint32_t hi = static_cast<uint32_t>(Mma<QT>::bits(x.z * inv)) | (static_cast<uint32_t>(Mma<QT>::bits(x.w * inv)) << 16);
-  *reinterpret_cast<uint2*>(dst) = make_uint2(lo, hi);
-  if (ln == 0 && p.lse) p.lse[orow] = lsum > 0.f ? (m - LIFT + log2f(lsum)) * LN2 : lsum == lsum ? -INFINITY : lsum;
+  store_row<QT>(static_cast<QT*>(p.out) + orow * D + 4 * ln, x, lsum);
+  if (ln == 0 && p.lse) p.lse[orow] = lse_of(m, lsum);
 }
-
-constexpr int SMS = 148;
 
 template <typename QT, int D, int CODE, int NG>
 int launch(const Params& p, const ic_paged_attn_args& a, cudaStream_t st) {
