@@ -205,13 +205,14 @@ __global__ void __launch_bounds__(NW * 32, ctas_per_sm(D, NG))
     }
     total = prefix[p.S];
   }
-  const int share = max((total + static_cast<int>(gridDim.x) - 1) / static_cast<int>(gridDim.x), p.min_share);
+  constexpr uint32_t CTAS = SMS * ctas_per_sm(D, NG);
+  const int share = max(static_cast<int>((static_cast<uint32_t>(total) + CTAS - 1) / CTAS), p.min_share);
   const int cta = blockIdx.x;
   const int64_t pos0 = static_cast<int64_t>(cta) * share;
   const int end = static_cast<int>(min(pos0 + share, static_cast<int64_t>(total)));
   float* part = p.ws;                                                    // [2 * ctas][ROWS][D]
-  float* part_stat = part + static_cast<size_t>(2) * gridDim.x * ROWS * D;  // [2 * ctas][ROWS][2]
-  Task* tasks = reinterpret_cast<Task*>(part_stat + static_cast<size_t>(2) * gridDim.x * ROWS * 2);
+  float* part_stat = part + static_cast<size_t>(2) * CTAS * ROWS * D;  // [2 * ctas][ROWS][2]
+  Task* tasks = reinterpret_cast<Task*>(part_stat + static_cast<size_t>(2) * CTAS * ROWS * 2);
   if (tid == 0) tasks[cta].valid = 0;
   if (pos0 >= end) return;
 
@@ -248,12 +249,13 @@ __global__ void __launch_bounds__(NW * 32, ctas_per_sm(D, NG))
       g.len = held_tokens(p, lo);
     }
     g.pages = max(1, (g.len + q8::PAGE - 1) / q8::PAGE);
-    const int tiles = (g.n_tok * p.G + ROWS - 1) / ROWS, at = pos - before, gi = at / g.pages;
+    const uint32_t tiles = static_cast<uint32_t>(g.n_tok * p.G + ROWS - 1) / ROWS, at = pos - before;
+    const uint32_t gi = at / static_cast<uint32_t>(g.pages), hh = tiles == 1 ? gi : gi / tiles;
     g.p0 = at - gi * g.pages;
     g.p1 = min(g.pages, g.p0 + (end - pos));
-    g.h = gi / tiles;
-    g.row0 = (gi - g.h * tiles) * ROWS;
-    g.mine = max(0, (g.p1 - g.p0 - warp + NW - 1) / NW);
+    g.h = hh;
+    g.row0 = (gi - hh * tiles) * ROWS;
+    g.mine = g.p1 - g.p0 > warp ? static_cast<uint32_t>(g.p1 - g.p0 - warp + NW - 1) / NW : 0;
     return g;
   };
   // Lane j holds page base + j of this warp: its id, then its K scale and the
@@ -404,12 +406,9 @@ __global__ void __launch_bounds__(NW * 32, ctas_per_sm(D, NG))
       if (page >= 0 && !dead) {
         const uint32_t kp = ring + st * 2 * L::PAGE_B, vp = kp + L::PAGE_B;
         const int tok0 = (seg.p0 + warp + NW * i) * q8::PAGE;
-        // two chains of products where one row tile would leave a single long one
-        float acc[NG][4], odd[NG == 1 ? 1 : NG][4];
+        float acc[NG][4];
 #pragma unroll
-        for (int nt = 0; nt < NG; ++nt)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) acc[nt][e] = odd[nt][e] = 0.f;
+        for (int nt = 0; nt < NG; ++nt) acc[nt][0] = acc[nt][1] = acc[nt][2] = acc[nt][3] = 0.f;
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
           const int chunk = D == 64 ? tq : (c >> 1) * 8 + 2 * tq + (c & 1);
@@ -422,12 +421,8 @@ __global__ void __launch_bounds__(NW * 32, ctas_per_sm(D, NG))
             q8::decode4_h2<CODE>(w1[j], a1, a3);
 #pragma unroll
             for (int nt = 0; nt < NG; ++nt)
-              Mma<__half>::run(NG == 1 && (j & 1) ? odd[nt] : acc[nt], a0, a1, a2, a3, qb[nt][c * 4 + j][0], qb[nt][c * 4 + j][1]);
+              Mma<__half>::run(acc[nt], a0, a1, a2, a3, qb[nt][c * 4 + j][0], qb[nt][c * 4 + j][1]);
           }
-        }
-        if (NG == 1) {
-#pragma unroll
-          for (int e = 0; e < 4; ++e) acc[0][e] += odd[0][e];
         }
         // V: tokens 2 tq, 2 tq + 1, 2 tq + 8, 2 tq + 9; this lane's D / 8 dims from D / 8 * g
         uint32_t t[4][W4];
@@ -603,79 +598,96 @@ __global__ void __launch_bounds__(NW * 32, ctas_per_sm(D, NG))
   }
 }
 
-// Joins the partials of the groups that lie in several shares: one CTA per
-// (CTA where such a group begins, row).  The weights of all partials come first
-// (a thread each), then eight subgroups of lanes add every eighth partial and
-// their sums are joined in order.
-template <typename QT, int D, int NG>
-__global__ void __launch_bounds__(8 * (D / 4)) join_kernel(const Params p, int ctas) {
-  constexpr int ROWS = 8 * NG, LN = D / 4, NT = 8 * LN, MAXP = 2 * SMS;
-  __shared__ float weight[MAXP];
-  __shared__ float4 sx[8][LN];
-  __shared__ float red[2][NT / 32];
+// Joins the partials of the groups that lie in several shares: for every CTA of
+// the streaming kernel (most have nothing to do and leave) one CTA, or several
+// with RPC rows of the tile each.  The weights of all partials first, a warp per
+// row; then the rows' elements, SUBS subgroups of threads with every SUBS-th
+// partial each, joined in order.
+constexpr int JT = 512;
+template <typename QT, int D, int NG, int RPC>
+__global__ void __launch_bounds__(JT) join_kernel(const Params p) {
+  constexpr int ROWS = 8 * NG, LN = D / 4, ITEMS = RPC * LN, SUBS = ITEMS >= JT ? 1 : JT / ITEMS;
+  constexpr int CTAS = SMS * ctas_per_sm(D, NG), PER = (CTAS + 31) / 32;
+  __shared__ float weight[RPC][CTAS + 1];
+  __shared__ float lsums[RPC], tops[RPC];
+  __shared__ float4 sx[SUBS > 1 ? JT : 1];
   grid_dependency_wait();
   grid_launch_dependents();
   const float* part = p.ws;
-  const float* part_stat = part + static_cast<size_t>(2) * ctas * ROWS * D;
-  const Task* tasks = reinterpret_cast<const Task*>(part_stat + static_cast<size_t>(2) * ctas * ROWS * 2);
-  const Task t = tasks[blockIdx.x];
+  const float* part_stat = part + static_cast<size_t>(2) * CTAS * ROWS * D;
+  const Task* tasks = reinterpret_cast<const Task*>(part_stat + static_cast<size_t>(2) * CTAS * ROWS * 2);
+  const int cta = blockIdx.x, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, row0 = blockIdx.y * RPC;
+  // partial i of the group that begins here: slot 0 or 1 of this CTA, then slot 0
+  // of each later one; lane i of a row's warp looks at partial i without waiting
+  // to hear how many there are
+  const auto stat_at = [&](int slot) {
+    return *reinterpret_cast<const float2*>(part_stat + (static_cast<size_t>(slot) * ROWS + row0 + warp) * 2);
+  };
+  float2 ml[PER], other = make_float2(0.f, 0.f);
+#pragma unroll
+  for (int k = 0; k < PER; ++k) ml[k] = make_float2(-INFINITY, 0.f);
+  if (warp < RPC && cta + lane < CTAS) ml[0] = stat_at(2 * (cta + lane));
+  if (warp < RPC && lane == 0) other = stat_at(2 * cta + 1);
+  const Task t = tasks[cta];
   if (!t.valid) return;
   int q_begin;
   const int rows = query_tokens(p, t.s, q_begin) * p.G;
-  const int row = blockIdx.y, r = t.tile * ROWS + row;
-  if (r >= rows) return;
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, sub = tid / LN, ln = tid % LN;
-  const int n = t.last_cta - static_cast<int>(blockIdx.x) + 1;
-  // partial i: the first share's, then slot 0 of each later one
-  const auto at = [&](int i) {
-    return (static_cast<size_t>(i == 0 ? t.first_slot : 2 * (blockIdx.x + i)) * ROWS + row);
-  };
-  constexpr int PER = (MAXP + NT - 1) / NT;
-  float2 ml[PER];
-  float m = -INFINITY, lsum = 0.f;
+  const int n = t.last_cta - cta + 1;
+  if (warp < RPC) {
+    if (lane == 0 && t.first_slot != 2 * cta) ml[0] = other;
+    if (lane >= n) ml[0].x = -INFINITY;
+    float m = -INFINITY, lsum = 0.f;
 #pragma unroll
-  for (int k = 0; k < PER; ++k) {
-    const int i = tid + k * NT;
-    ml[k] = make_float2(-INFINITY, 0.f);
-    if (i < n) ml[k] = *reinterpret_cast<const float2*>(part_stat + at(i) * 2);
-    m = fmaxf(m, ml[k].x);
+    for (int k = 0; k < PER; ++k) {
+      if (k > 0 && lane + 32 * k < n) ml[k] = stat_at(2 * (cta + lane + 32 * k));
+    }
+#pragma unroll
+    for (int k = 0; k < PER; ++k) m = fmaxf(m, ml[k].x);
+    m = warp_max(m);
+#pragma unroll
+    for (int k = 0; k < PER; ++k) {
+      if (lane + 32 * k < n) {
+        const float f = ml[k].x == -INFINITY ? 0.f : tc::ex2(ml[k].x - m);
+        weight[warp][lane + 32 * k] = f;
+        lsum = fmaf(ml[k].y, f, lsum);
+      }
+    }
+    lsum = warp_sum(lsum);
+    if (lane == 0) {
+      lsums[warp] = lsum;
+      tops[warp] = m;
+    }
   }
-  m = warp_max(m);
-  if (lane == 0) red[0][warp] = m;
   __syncthreads();
-#pragma unroll
-  for (int i = 0; i < NT / 32; ++i) m = fmaxf(m, red[0][i]);
-#pragma unroll
-  for (int k = 0; k < PER; ++k) {
-    const int i = tid + k * NT;
-    const float f = ml[k].x == -INFINITY ? 0.f : tc::ex2(ml[k].x - m);
-    if (i < n) weight[i] = f;
-    lsum = fmaf(ml[k].y, f, lsum);
-  }
-  lsum = warp_sum(lsum);
-  if (lane == 0) red[1][warp] = lsum;
-  __syncthreads();
-  float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int e = tid; e < ITEMS * SUBS; e += JT) {
+    const int sub = e / ITEMS, er = e % ITEMS / LN, d0 = e % LN * 4, r = t.tile * ROWS + row0 + er;
+    const auto load = [&](int i) {
+      const size_t at = static_cast<size_t>(i == 0 ? t.first_slot : 2 * (cta + i)) * ROWS + row0 + er;
+      return *reinterpret_cast<const float4*>(part + at * D + d0);
+    };
+    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 8
-  for (int i = sub; i < n; i += 8) {
-    const float4 u = *reinterpret_cast<const float4*>(part + at(i) * D + 4 * ln);
-    const float f = weight[i];
-    x.x = fmaf(u.x, f, x.x); x.y = fmaf(u.y, f, x.y); x.z = fmaf(u.z, f, x.z); x.w = fmaf(u.w, f, x.w);
-  }
-  sx[sub][ln] = x;
-  __syncthreads();
-  if (sub != 0) return;
-  lsum = 0.f;
+    for (int i = sub; i < n; i += SUBS) {
+      const float4 u = load(i);
+      const float f = weight[er][i];
+      x.x = fmaf(u.x, f, x.x); x.y = fmaf(u.y, f, x.y); x.z = fmaf(u.z, f, x.z); x.w = fmaf(u.w, f, x.w);
+    }
+    if (SUBS > 1) {
+      sx[tid] = x;
+      __syncthreads();  // ITEMS * SUBS = JT: every thread comes here once
+      if (sub != 0) return;
 #pragma unroll
-  for (int i = 0; i < NT / 32; ++i) lsum += red[1][i];
-#pragma unroll
-  for (int i = 1; i < 8; ++i) {
-    const float4 u = sx[i][ln];
-    x.x += u.x; x.y += u.y; x.z += u.z; x.w += u.w;
+      for (int i = 1; i < SUBS; ++i) {
+        const float4 u = sx[tid + i * ITEMS];
+        x.x += u.x; x.y += u.y; x.z += u.z; x.w += u.w;
+      }
+    }
+    if (r < rows) {
+      const int64_t orow = static_cast<int64_t>(q_begin + r / p.G) * p.Hq + t.h * p.G + r % p.G;
+      store_row<QT>(static_cast<QT*>(p.out) + orow * D + d0, x, lsums[er]);
+      if (d0 == 0 && p.lse) p.lse[orow] = lse_of(tops[er], lsums[er]);
+    }
   }
-  const int64_t orow = static_cast<int64_t>(q_begin + r / p.G) * p.Hq + t.h * p.G + r % p.G;
-  store_row<QT>(static_cast<QT*>(p.out) + orow * D + 4 * ln, x, lsum);
-  if (ln == 0 && p.lse) p.lse[orow] = lse_of(m, lsum);
 }
 
 template <typename QT, int D, int CODE, int NG>
@@ -689,14 +701,17 @@ int launch(const Params& p, const ic_paged_attn_args& a, cudaStream_t st) {
   const int smem = Layout<D, NG>::bytes(p.S);
   if ((rc = ensure_dynamic_smem(kern, smem, &limit)) != IC_OK) return rc;
   Params params = p;
-  int ctas = SMS * ctas_per_sm(D, NG);
+  constexpr int ctas = SMS * ctas_per_sm(D, NG);
   void* args[] = {&mk, &mv, &params};
   if ((rc = launch_pdl(reinterpret_cast<const void*>(kern), dim3(ctas), dim3(NW * 32), smem, st, args,
                        "paged_attention (stream)")) != IC_OK)
     return rc;
-  void* jargs[] = {&params, &ctas};
-  return launch_pdl(reinterpret_cast<const void*>(join_kernel<QT, D, NG>), dim3(ctas, 8 * NG), dim3(8 * (D / 4)), 0, st,
-                    jargs, "paged_attention (join)");
+  // Few groups mean many partials each: then two rows per CTA.
+  void* jargs[] = {&params};
+  const bool few = p.S * p.H <= 16;
+  const void* join = few ? reinterpret_cast<const void*>(join_kernel<QT, D, NG, 2>)
+                         : reinterpret_cast<const void*>(join_kernel<QT, D, NG, 8 * NG>);
+  return launch_pdl(join, dim3(ctas, few ? 4 * NG : 1), dim3(JT), 0, st, jargs, "paged_attention (join)");
 }
 
 template <typename QT, int D, int CODE>
