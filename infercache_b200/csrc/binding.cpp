@@ -8,6 +8,7 @@
 // _lib.raise_for, which every other binding uses too.
 #include <ATen/ATen.h>
 #include <ATen/cuda/CUDAContext.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -127,6 +128,11 @@ bool rows16(const Tensor& t) {
 }
 bool aligned16(const Tensor& t) { return reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0; }
 
+// An uninitialised contiguous tensor on `dev` (made current by the caller).
+Tensor fresh(at::IntArrayRef shape, at::ScalarType type, c10::Device dev) {
+  return at::detail::empty_cuda(shape, type, dev, std::nullopt);
+}
+
 struct Cache {
   c10::Device dev{c10::kCPU};
   int64_t dims, L, H, n, D;
@@ -229,10 +235,9 @@ PyObject* py_page_plan(PyObject*, PyObject* const* a, Py_ssize_t n) {
     x.free_count = count_p;
     x.dev_status = status_word(name, a[7], dev);
     c10::cuda::CUDAGuard guard(dev);
-    const auto i32 = lens.options();
-    Tensor q_start = at::empty({S + 1}, i32), slots = at::empty({total}, i32);
-    Tensor positions = at::empty({total}, i32.dtype(at::kLong)), work = at::empty({2 * S + 1}, i32);
-    Tensor lens_out = commit ? lens : at::empty({S}, i32), count_out = commit ? count : at::empty({1}, i32);
+    Tensor q_start = fresh({S + 1}, at::kInt, dev), slots = fresh({total}, at::kInt, dev);
+    Tensor positions = fresh({total}, at::kLong, dev), work = fresh({2 * S + 1}, at::kInt, dev);
+    Tensor lens_out = commit ? lens : fresh({S}, at::kInt, dev), count_out = commit ? count : fresh({1}, at::kInt, dev);
     x.q_start = static_cast<int32_t*>(q_start.data_ptr());
     x.slots = static_cast<int32_t*>(slots.data_ptr());
     x.positions = static_cast<int64_t*>(positions.data_ptr());
@@ -334,9 +339,8 @@ PyObject* py_page_read(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (none(a[6])) {
       const int64_t code = integer(a[5]);
       const auto type = code == IC_F32 ? at::kFloat : code == IC_F16 ? at::kHalf : at::kBFloat16;
-      const auto opt = c.k->options().dtype(type);
-      k = at::empty(shape, opt);
-      v = at::empty(shape, opt);
+      k = fresh(shape, type, c.dev);
+      v = fresh(shape, type, c.dev);
     } else {
       k = tensor(a[6], name, "out");
       v = tensor(a[7], name, "out");
@@ -391,7 +395,7 @@ PyObject* py_paged_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
     c10::cuda::CUDAGuard guard(c.dev);
     Tensor out, lse;
     if (none(a[10])) {
-      out = at::empty(q.sizes(), q.options());
+      out = fresh(q.sizes(), type, c.dev);
     } else {
       out = tensor(a[10], name, "out");
       if (out.sizes() != q.sizes() || out.scalar_type() != type || out.device() != c.dev || !out.is_contiguous() ||
@@ -399,7 +403,7 @@ PyObject* py_paged_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
         bad(name, "out must be a contiguous, 16-byte aligned tensor like q");
     }
     const bool want_lse = PyObject_IsTrue(a[11]) == 1;
-    if (want_lse) lse = at::empty({N, Hq}, c.ks->options());
+    if (want_lse) lse = fresh({N, Hq}, at::kFloat, c.dev);
     if (N > 0 && S > 0) {
       if (!rows16(q)) q = q.clone(at::MemoryFormat::Contiguous);
       x.q = q.data_ptr();
@@ -426,7 +430,7 @@ PyObject* py_paged_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
       Tensor work;
       x.workspace_bytes = ic_paged_attention_workspace(&x);
       if (x.workspace_bytes > 0) {
-        work = at::empty({x.workspace_bytes / 4 + 1}, c.ks->options());
+        work = fresh({x.workspace_bytes}, at::kByte, c.dev);
         x.workspace = work.data_ptr();
       }
       check_status(ic_paged_attention(&x, at::cuda::getCurrentCUDAStream(c.dev.index()).stream()), "ic_paged_attention");
@@ -468,7 +472,7 @@ PyObject* py_process_logits(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (x.stride(1) != 1 || (S > 1 && x.stride(0) < V)) x = x.contiguous();
     Tensor out;
     if (none(a[11])) {
-      out = at::empty({S, V}, x.options().dtype(at::kFloat));
+      out = fresh({S, V}, at::kFloat, dev);
     } else {
       out = tensor(a[11], name, "out");
       if (out.scalar_type() != at::kFloat || out.sizes() != x.sizes() || out.device() != dev || out.stride(1) != 1 ||
