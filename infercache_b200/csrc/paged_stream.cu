@@ -126,6 +126,20 @@ __device__ __forceinline__ uint32_t max_magnitude(uint32_t m, const uint4& v) { 
   return m;
 }
 
+__device__ __forceinline__ float2 ld_cluster2(uint32_t addr) {
+  float2 v;
+  asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(addr) : "memory");
+  return v;
+}
+__device__ __forceinline__ float4 ld_cluster4(uint32_t addr) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+               : "r"(addr)
+               : "memory");
+  return v;
+}
+
 // Four finished elements x / l; no key at all gives zeros, NaN stays NaN.
 template <typename QT>
 __device__ __forceinline__ void store_row(QT* dst, const float4& x, float l) {
@@ -139,7 +153,8 @@ __device__ __forceinline__ float lse_of(float m, float l) {
   return l > 0.f ? (m - LIFT + log2f(l)) * LN2 : l == l ? -INFINITY : l;
 }
 
-template <typename QT, int D, int CODE, int NG>
+// GROUPED: one cluster of CTAs per group instead of shares of the line.
+template <typename QT, int D, int CODE, int NG, bool GROUPED>
 __global__ void __launch_bounds__(NW * 32, ctas_per_sm(D, NG))
     stream_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv, const Params p) {
   using L = Layout<D, NG>;
@@ -153,6 +168,8 @@ __global__ void __launch_bounds__(NW * 32, ctas_per_sm(D, NG))
   int32_t* prefix = reinterpret_cast<int32_t*>(smem + L::PREFIX);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int g = lane >> 2, tq = lane & 3;
+  const int CL = GROUPED ? p.cluster : 1, rank = GROUPED ? static_cast<int>(cluster_ctarank()) : 0;
+  const int gw = rank * NW + warp, stride = NW * CL;  // this warp among those of a segment
 
   if (tid < NW * ST) {
     mbar_init(bars + tid, 1);
@@ -170,7 +187,8 @@ __global__ void __launch_bounds__(NW * 32, ctas_per_sm(D, NG))
     tok = query_tokens(p, x, begin);
     len = held_tokens(p, x);
     const int rows = tok * p.G;
-    return rows <= p.few_rows ? (rows + ROWS - 1) / ROWS * p.H * max(1, (len + q8::PAGE - 1) / q8::PAGE) : 0;
+    const int pages = GROUPED ? 1 : max(1, (len + q8::PAGE - 1) / q8::PAGE);
+    return rows <= p.few_rows ? (rows + ROWS - 1) / ROWS * p.H * pages : 0;
   };
   if (lanes) {
     if (lane < p.S) l_upto = units_of(lane, l_begin, l_tok, l_len);
@@ -206,15 +224,15 @@ __global__ void __launch_bounds__(NW * 32, ctas_per_sm(D, NG))
     total = prefix[p.S];
   }
   constexpr uint32_t CTAS = SMS * ctas_per_sm(D, NG);
-  const int share = max(static_cast<int>((static_cast<uint32_t>(total) + CTAS - 1) / CTAS), p.min_share);
-  const int cta = blockIdx.x;
+  const int share = GROUPED ? 1 : max(static_cast<int>((static_cast<uint32_t>(total) + CTAS - 1) / CTAS), p.min_share);
+  const int cta = GROUPED ? blockIdx.x / CL : blockIdx.x;
   const int64_t pos0 = static_cast<int64_t>(cta) * share;
   const int end = static_cast<int>(min(pos0 + share, static_cast<int64_t>(total)));
-  float* part = p.ws;                                                    // [2 * ctas][ROWS][D]
-  float* part_stat = part + static_cast<size_t>(2) * CTAS * ROWS * D;  // [2 * ctas][ROWS][2]
+  float* part = p.ws;                                                  // [2 * CTAS][ROWS][D]
+  float* part_stat = part + static_cast<size_t>(2) * CTAS * ROWS * D;  // [2 * CTAS][ROWS][2]
   Task* tasks = reinterpret_cast<Task*>(part_stat + static_cast<size_t>(2) * CTAS * ROWS * 2);
-  if (tid == 0) tasks[cta].valid = 0;
-  if (pos0 >= end) return;
+  if (!GROUPED && tid == 0) tasks[cta].valid = 0;
+  if (pos0 >= end) return;  // GROUPED: a whole cluster
 
   const uint32_t ring = smem_addr(smem) + warp * (ST * 2 * L::PAGE_B);
   uint64_t* wbar = bars + warp * ST;
@@ -223,7 +241,7 @@ __global__ void __launch_bounds__(NW * 32, ctas_per_sm(D, NG))
   int st = 0;            // stage of the next page to be consumed
 
   // A segment: session s, KV head h, row tile, pages p0 .. p1 of the group; this
-  // warp's are p0 + warp + NW * i, i < mine.
+  // warp's are p0 + gw + stride * i, i < mine.
   struct Seg {
     int s, h, q_begin, n_tok, len, row0, pages, p0, p1, mine;
   };
@@ -250,19 +268,19 @@ __global__ void __launch_bounds__(NW * 32, ctas_per_sm(D, NG))
     }
     g.pages = max(1, (g.len + q8::PAGE - 1) / q8::PAGE);
     const uint32_t tiles = static_cast<uint32_t>(g.n_tok * p.G + ROWS - 1) / ROWS, at = pos - before;
-    const uint32_t gi = at / static_cast<uint32_t>(g.pages), hh = tiles == 1 ? gi : gi / tiles;
-    g.p0 = at - gi * g.pages;
-    g.p1 = min(g.pages, g.p0 + (end - pos));
+    const uint32_t gi = GROUPED ? at : at / static_cast<uint32_t>(g.pages), hh = tiles == 1 ? gi : gi / tiles;
+    g.p0 = GROUPED ? 0 : at - gi * g.pages;
+    g.p1 = GROUPED ? g.pages : min(g.pages, g.p0 + (end - pos));
     g.h = hh;
     g.row0 = (gi - hh * tiles) * ROWS;
-    g.mine = g.p1 - g.p0 > warp ? static_cast<uint32_t>(g.p1 - g.p0 - warp + NW - 1) / NW : 0;
+    g.mine = g.p1 - g.p0 > gw ? static_cast<uint32_t>(g.p1 - g.p0 - gw + stride - 1) / static_cast<uint32_t>(stride) : 0;
     return g;
   };
   // Lane j holds page base + j of this warp: its id, then its K scale and the
   // logarithm and reciprocal of its V scale (both at least 2^-100, so a zero
   // scale stays harmless).
   const auto fetch_id = [&](const Seg& g, int base) {
-    const int i = base + lane, pg = g.p0 + warp + NW * i;
+    const int i = base + lane, pg = g.p0 + gw + stride * i;
     int id = -1;
     if (i < g.mine && pg * q8::PAGE < g.len) {
       id = p.table[static_cast<int64_t>(g.s) * p.width + pg];
@@ -405,7 +423,7 @@ __global__ void __launch_bounds__(NW * 32, ctas_per_sm(D, NG))
       }
       if (page >= 0 && !dead) {
         const uint32_t kp = ring + st * 2 * L::PAGE_B, vp = kp + L::PAGE_B;
-        const int tok0 = (seg.p0 + warp + NW * i) * q8::PAGE;
+        const int tok0 = (seg.p0 + gw + stride * i) * q8::PAGE;
         float acc[NG][4];
 #pragma unroll
         for (int nt = 0; nt < NG; ++nt) acc[nt][0] = acc[nt][1] = acc[nt][2] = acc[nt][3] = 0.f;
@@ -519,7 +537,7 @@ __global__ void __launch_bounds__(NW * 32, ctas_per_sm(D, NG))
 
     // ---- the next segment's first pages are on their way while this one is joined ------
     const int next_pos = pos + seg.p1 - seg.p0;
-    const bool more = next_pos < end;
+    const bool more = !GROUPED && next_pos < end;
     Seg nseg;
     int nid = -1;
     if (more) {
@@ -536,6 +554,8 @@ __global__ void __launch_bounds__(NW * 32, ctas_per_sm(D, NG))
 
     // ---- join the warps, 8 rows at a time ----------------------------------------------
     float* wo = reinterpret_cast<float*>(smem + L::MERGE);
+    float* cx = reinterpret_cast<float*>(smem);  // GROUPED: [8][D] in the ring, which is done, and [8][2] behind it
+    float* cs = cx + 8 * D;
     const bool whole = seg.p0 == 0 && seg.p1 == seg.pages;
     const int slot = 2 * cta + (pos == pos0 ? 0 : 1);
 #pragma unroll
@@ -570,7 +590,10 @@ __global__ void __launch_bounds__(NW * 32, ctas_per_sm(D, NG))
           x.x = fmaf(u.x, f, x.x); x.y = fmaf(u.y, f, x.y); x.z = fmaf(u.z, f, x.z); x.w = fmaf(u.w, f, x.w);
         }
         const size_t prow = static_cast<size_t>(slot) * ROWS + nt * 8 + row;
-        if (!whole) {
+        if (GROUPED) {  // this CTA's part, for the cluster to read
+          *reinterpret_cast<float4*>(cx + row * D + d0) = x;
+          if (d0 == 0) *reinterpret_cast<float2*>(cs + row * 2) = make_float2(m, lsum);
+        } else if (!whole) {
           *reinterpret_cast<float4*>(part + prow * D + d0) = x;
           if (d0 == 0) *reinterpret_cast<float2*>(part_stat + prow * 2) = make_float2(m, lsum);
         } else if (r < rows) {
@@ -580,6 +603,39 @@ __global__ void __launch_bounds__(NW * 32, ctas_per_sm(D, NG))
         }
       }
       __syncthreads();
+    }
+    if (GROUPED) {
+      // Every CTA's 8 rows lie in its shared memory; CTA j finishes rows j, j + CL,
+      // ..., a warp each, adding the parts in the CTAs' order.
+      cluster_arrive_release();
+      cluster_wait_acquire();
+      const int row = rank + warp * CL, r = row0 + row;
+      if (row < 8 && r < rows) {
+        const uint32_t sa = smem_addr(cs + row * 2), xa = smem_addr(cx + row * D);
+        float m = -INFINITY;
+        for (int j = 0; j < CL; ++j) m = fmaxf(m, ld_cluster2(map_shared(sa, j)).x);
+        float lsum = 0.f;
+        for (int j = 0; j < CL; ++j) {
+          const float2 v = ld_cluster2(map_shared(sa, j));
+          lsum = fmaf(v.y, v.x == -INFINITY ? 0.f : tc::ex2(v.x - m), lsum);
+        }
+        const int64_t orow = static_cast<int64_t>(seg.q_begin + r / p.G) * p.Hq + h * p.G + r % p.G;
+#pragma unroll
+        for (int d0 = lane * 4; d0 < D; d0 += 128) {
+          float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+          for (int j = 0; j < CL; ++j) {
+            const float mj = ld_cluster2(map_shared(sa, j)).x;
+            const float f = mj == -INFINITY ? 0.f : tc::ex2(mj - m);
+            const float4 u = ld_cluster4(map_shared(xa + d0 * 4, j));
+            x.x = fmaf(u.x, f, x.x); x.y = fmaf(u.y, f, x.y); x.z = fmaf(u.z, f, x.z); x.w = fmaf(u.w, f, x.w);
+          }
+          store_row<QT>(static_cast<QT*>(p.out) + orow * D + d0, x, lsum);
+        }
+        if (lane == 0 && p.lse) p.lse[orow] = lse_of(m, lsum);
+      }
+      cluster_arrive_release();  // nobody leaves while its rows are read
+      cluster_wait_acquire();
+      break;
     }
     if (tid == 0 && seg.p0 == 0 && seg.p1 < seg.pages) {  // this CTA holds the group's first page, not its last
       Task t;
@@ -690,17 +746,59 @@ __global__ void __launch_bounds__(JT) join_kernel(const Params p) {
   }
 }
 
+// At most this many groups of 8 rows, whatever the sessions' counts.
+int64_t group_bound(const ic_paged_attn_args& a) {
+  const int64_t G = a.num_q_heads / a.num_kv_heads, n = a.num_q_tokens;
+  return std::min<int64_t>(n * ((G + 7) / 8), n * G / 8 + std::min<int64_t>(a.num_sessions, n)) * a.num_kv_heads;
+}
+// CTAs per group when each group gets a cluster of its own, 0 for shares of the
+// line.  A cluster joins its parts through distributed shared memory, without
+// the 3 to 4 us of a second kernel, but a group is then split over no more than
+// 8 CTAs: so only while all clusters run at once and the table's width leaves a
+// CTA at most MAX_CTA_PAGES pages.
+constexpr int MAX_CTA_PAGES = 96;
+int cluster_size(const ic_paged_attn_args& a, int per_sm) {
+  const int64_t groups = group_bound(a);
+  for (int cl = 8; cl >= 2; cl /= 2)
+    if (groups * cl <= SMS * per_sm) return a.table_width <= MAX_CTA_PAGES * cl ? cl : 0;
+  return 0;
+}
+
 template <typename QT, int D, int CODE, int NG>
 int launch(const Params& p, const ic_paged_attn_args& a, cudaStream_t st) {
   CUtensorMap mk, mv;
   int rc;
   if ((rc = page_map(&mk, a.k, a.pool_tokens, p.H, D)) != IC_OK) return rc;
   if ((rc = page_map(&mv, a.v, a.pool_tokens, p.H, D)) != IC_OK) return rc;
-  auto kern = stream_kernel<QT, D, CODE, NG>;
-  static PerDeviceLimit limit;
-  const int smem = Layout<D, NG>::bytes(p.S);
-  if ((rc = ensure_dynamic_smem(kern, smem, &limit)) != IC_OK) return rc;
   Params params = p;
+  const int smem = Layout<D, NG>::bytes(p.S);
+  if constexpr (NG == 1) {
+    const int cl = cluster_size(a, ctas_per_sm(D, NG));
+    if (cl > 0) {
+      static PerDeviceLimit grouped_limit;
+      auto kern = stream_kernel<QT, D, CODE, NG, true>;
+      if ((rc = ensure_dynamic_smem(kern, smem, &grouped_limit)) != IC_OK) return rc;
+      params.cluster = cl;
+      cudaLaunchConfig_t cfg = {};
+      cfg.gridDim = dim3(static_cast<unsigned>(group_bound(a) * cl));
+      cfg.blockDim = dim3(NW * 32);
+      cfg.dynamicSmemBytes = smem;
+      cfg.stream = st;
+      cudaLaunchAttribute attr[2];
+      attr[0].id = cudaLaunchAttributeClusterDimension;
+      attr[0].val.clusterDim.x = cl;
+      attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+      attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+      attr[1].val.programmaticStreamSerializationAllowed = 1;
+      cfg.attrs = attr;
+      cfg.numAttrs = 2;
+      cudaLaunchKernelEx(&cfg, kern, mk, mv, params);
+      return launch_status("paged_attention (stream, grouped)");
+    }
+  }
+  auto kern = stream_kernel<QT, D, CODE, NG, false>;
+  static PerDeviceLimit limit;
+  if ((rc = ensure_dynamic_smem(kern, smem, &limit)) != IC_OK) return rc;
   constexpr int ctas = SMS * ctas_per_sm(D, NG);
   void* args[] = {&mk, &mv, &params};
   if ((rc = launch_pdl(reinterpret_cast<const void*>(kern), dim3(ctas), dim3(NW * 32), smem, st, args,

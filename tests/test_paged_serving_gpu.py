@@ -305,6 +305,27 @@ def test_attention_shares(codes, S, top):
     check_attention(attention_inputs(S, lens, [min(2, n) for n in lens], 2, 5, 64, codes, torch.float16))
 
 
+@pytest.mark.parametrize("S", [1, 5, 40, 70])
+@pytest.mark.parametrize("G,D", [(8, 128), (5, 64), (1, 256)])
+def test_attention_whatever_the_table_holds(S, G, D):
+    """Narrow tables give every group a cluster of CTAs (of 8, 4, 2), wide ones equal
+    shares of all pages: the same sessions through both, and with sessions
+    that have nothing to ask or to attend over."""
+    rng = np.random.default_rng(S)
+    lens = rng.integers(0, 1500, S).tolist()
+    lens[0] = 1500
+    counts = [1 if n else int(rng.integers(0, 2)) for n in lens]
+    counts[-1] = 1
+    x = attention_inputs(S + G, lens, counts, 2, G, D, torch.float8_e4m3fn, torch.float16)
+    check_attention(x, max_count=1)
+    wide = torch.full((S, 2000), -1, dtype=torch.int32, device="cuda")
+    wide[:, :x[5].shape[1]] = x[5]
+    check_attention(x[:5] + (wide,) + x[6:], max_count=1)
+    # fewer tokens announced than some session has
+    lens, counts = [n + 20 for n in lens], [c * 9 for c in counts]
+    check_attention(attention_inputs(S + G + 1, lens, counts, 2, G, D, torch.int8, torch.bfloat16), max_count=1)
+
+
 @pytest.mark.parametrize("codes", CODES)
 def test_attention_scales_far_apart(codes):
     """Page scales over 2^+-20 for V, scores of hundreds, q at bf16's extremes."""
