@@ -680,8 +680,9 @@ int ic_page_read_q8(const ic_page_q8_args* a, void* stream);
  * 16]; q has strides (elements), out is [num_q_tokens, Hq, D] contiguous in
  * q's dtype (fp16 / bf16); D is 64, 128 or 256.  max_count bounds the query
  * tokens of one session (it steers the choice of kernel only: a session with
- * more is still computed).  workspace: ic_paged_attention_workspace(a) bytes,
- * 16-byte aligned, not shared by calls that may overlap. */
+ * more is still computed).  workspace: ic_paged_attention_workspace(a) bytes
+ * (NULL when that is 0), 16-byte aligned, not shared by calls that may
+ * overlap. */
 typedef struct ic_paged_attn_args {
   const void* q;
   void* out;
@@ -705,7 +706,7 @@ typedef struct ic_paged_attn_args {
   float scale;
 } ic_paged_attn_args;
 int ic_paged_attention(const ic_paged_attn_args* a, void* stream);
-/* bytes of workspace that the call needs (0 for arguments it would refuse) */
+/* bytes of workspace that the call needs (0: none, or it would be refused) */
 int64_t ic_paged_attention_workspace(const ic_paged_attn_args* a);
 
 /* ---- Penalties, biases and grammar masks on logits --------------------------------

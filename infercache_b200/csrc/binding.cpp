@@ -133,6 +133,15 @@ Tensor fresh(at::IntArrayRef shape, at::ScalarType type, c10::Device dev) {
   return at::detail::empty_cuda(shape, type, dev, std::nullopt);
 }
 
+// `shape` elements of a one-dimensional tensor from `offset` on, as a tensor of
+// its own over the same memory.
+Tensor part_of(const Tensor& base, int64_t offset, int64_t shape) {
+  Tensor t = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(base.storage()), base.key_set(), base.dtype());
+  t.unsafeGetTensorImpl()->set_storage_offset(offset);
+  t.unsafeGetTensorImpl()->set_sizes_contiguous({shape});
+  return t;
+}
+
 struct Cache {
   c10::Device dev{c10::kCPU};
   int64_t dims, L, H, n, D;
@@ -235,15 +244,17 @@ PyObject* py_page_plan(PyObject*, PyObject* const* a, Py_ssize_t n) {
     x.free_count = count_p;
     x.dev_status = status_word(name, a[7], dev);
     c10::cuda::CUDAGuard guard(dev);
-    Tensor q_start = fresh({S + 1}, at::kInt, dev), slots = fresh({total}, at::kInt, dev);
-    Tensor positions = fresh({total}, at::kLong, dev), work = fresh({2 * S + 1}, at::kInt, dev);
-    Tensor lens_out = commit ? lens : fresh({S}, at::kInt, dev), count_out = commit ? count : fresh({1}, at::kInt, dev);
+    // the small results and the workspace share an allocation
+    const Tensor small = fresh({4 * S + 3}, at::kInt, dev);
+    Tensor slots = fresh({total}, at::kInt, dev), positions = fresh({total}, at::kLong, dev);
+    Tensor q_start = part_of(small, 0, S + 1);
+    Tensor lens_out = commit ? lens : part_of(small, S + 1, S), count_out = commit ? count : part_of(small, 2 * S + 1, 1);
     x.q_start = static_cast<int32_t*>(q_start.data_ptr());
     x.slots = static_cast<int32_t*>(slots.data_ptr());
     x.positions = static_cast<int64_t*>(positions.data_ptr());
     x.lens_out = static_cast<int32_t*>(lens_out.data_ptr());
     x.free_count_out = static_cast<int32_t*>(count_out.data_ptr());
-    x.workspace = static_cast<int32_t*>(work.data_ptr());
+    x.workspace = static_cast<int32_t*>(small.data_ptr()) + 2 * S + 2;
     x.num_sessions = static_cast<int32_t>(S);
     x.width = static_cast<int32_t>(std::min<int64_t>(W, 0x7fffffff));
     x.total = static_cast<int32_t>(total);

@@ -109,16 +109,15 @@ int page_map(CUtensorMap* m, const void* codes, int64_t pool_tokens, int heads, 
 }  // namespace ic
 
 extern "C" int64_t ic_paged_attention_workspace(const ic_paged_attn_args* a) {
-  if (ic::paged::check(a) != IC_OK) return 0;
-  const int64_t G = a->num_q_heads / a->num_kv_heads;
-  return ic::paged::stream_workspace(a->head_dim, ic::paged::stream_rows(static_cast<int64_t>(a->max_count) * G));
+  return ic::paged::check(a) == IC_OK ? ic::paged::stream_workspace(*a) : 0;
 }
 
 extern "C" int ic_paged_attention(const ic_paged_attn_args* a, void* stream) {
   using namespace ic;
   int rc = paged::check(a);
   if (rc != IC_OK) return rc;
-  if (!a->workspace || !paged::aligned16(a->workspace) || a->workspace_bytes < ic_paged_attention_workspace(a)) {
+  const int64_t need = paged::stream_workspace(*a);
+  if (need > 0 && (!a->workspace || !paged::aligned16(a->workspace) || a->workspace_bytes < need)) {
     set_last_error("paged_attention: workspace missing, misaligned or too small");
     return IC_ERR_INVALID_ARG;
   }

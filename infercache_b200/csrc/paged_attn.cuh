@@ -56,7 +56,7 @@ int launch_stream(const Params& p, const ic_paged_attn_args& a, cudaStream_t st)
 int launch_tile(const Params& p, const ic_paged_attn_args& a, cudaStream_t st);
 // Rows per tile of the streaming kernel: 8 where they hold a whole session's.
 inline int stream_rows(int64_t max_rows) { return max_rows <= 8 ? 8 : 16; }
-int64_t stream_workspace(int head_dim, int rows_per_tile);
+int64_t stream_workspace(const ic_paged_attn_args& a);  // bytes, 0 when the call needs none
 
 }  // namespace paged
 }  // namespace ic

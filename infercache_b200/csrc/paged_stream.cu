@@ -831,9 +831,12 @@ int launch_dim(const Params& p, const ic_paged_attn_args& a, cudaStream_t st, bo
 
 }  // namespace
 
-int64_t stream_workspace(int head_dim, int rows_per_tile) {
-  const int64_t ctas = SMS * ctas_per_sm(head_dim, rows_per_tile / 8);
-  return 2 * ctas * rows_per_tile * (head_dim + 2) * 4 + ctas * static_cast<int64_t>(sizeof(Task));
+int64_t stream_workspace(const ic_paged_attn_args& a) {
+  const int rows = stream_rows(static_cast<int64_t>(a.max_count) * (a.num_q_heads / a.num_kv_heads));
+  const int per_sm = ctas_per_sm(a.head_dim, rows / 8);
+  if (rows == 8 && cluster_size(a, per_sm) > 0) return 0;
+  const int64_t ctas = SMS * per_sm;
+  return 2 * ctas * rows * (a.head_dim + 2) * 4 + ctas * static_cast<int64_t>(sizeof(Task));
 }
 
 int launch_stream(const Params& p, const ic_paged_attn_args& a, cudaStream_t st) {

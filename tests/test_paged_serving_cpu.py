@@ -71,9 +71,9 @@ def test_page_rows_refusals(lib, p, name):
 
 def test_attention_refusals(lib, p):
     base = dict(q=p, out=p, k=p, v=p, k_scale=p, v_scale=p, block_table=p, lens=p, q_start=p, workspace=p,
-                workspace_bytes=1 << 40, pool_tokens=64, q_stride_t=1024, q_stride_h=128, num_sessions=2, table_width=4,
+                workspace_bytes=1 << 40, pool_tokens=64, q_stride_t=1024, q_stride_h=128, num_sessions=2, table_width=4000,
                 num_q_tokens=3, max_count=3, num_q_heads=8, num_kv_heads=2, head_dim=128, q_dtype=_lib.IC_F16,
-                code_dtype=_lib.IC_E4M3, scale=0.1)
+                code_dtype=_lib.IC_E4M3, scale=0.1)  # a wide table: the shares of a line, which need workspace
     cls = _lib.ic_paged_attn_args
     need = lib.ic_paged_attention_workspace(ctypes.byref(cls(**base)))
     assert need > 0 and lib.ic_paged_attention_workspace(None) == 0
@@ -84,6 +84,7 @@ def test_attention_refusals(lib, p):
                    dict(code_dtype=_lib.IC_F16), dict(q=p + 8), dict(out=p + 2), dict(k=p + 4), dict(workspace=p + 4),
                    dict(workspace_bytes=need - 1), dict(table_width=(1 << 26) + 1)]):
         expect(lib, "ic_paged_attention", cls, base, bad)
+    assert lib.ic_paged_attention_workspace(ctypes.byref(cls(**{**base, "table_width": 4, "max_count": 1}))) == 0
     for bad in (dict(head_dim=96), dict(num_sessions=4097), dict(table_width=1 << 26, num_q_tokens=1000)):
         expect(lib, "ic_paged_attention", cls, base, bad, UNSUPPORTED)
         assert lib.ic_paged_attention_workspace(ctypes.byref(cls(**{**base, **bad}))) == 0
