@@ -140,9 +140,24 @@ __global__ void __launch_bounds__(LT) logits_kernel(const ic_logits_args a) {
     uint32_t first = 0;
 #pragma unroll
     for (int j = 0; j < AHEAD; ++j) first |= static_cast<uint32_t>(count(tid + LT * j, ahead[j])) << j;
+    // one place on the list's end per warp, not per id: the ends' counter would
+    // serialise the CTA
+    int upto = __popc(first);
 #pragma unroll
-    for (int j = 0; j < AHEAD; ++j)
-      if ((first >> j) & 1u) push(ahead[j]);
+    for (int o = 1; o < 32; o <<= 1) {
+      const int u = __shfl_up_sync(FULL_MASK, upto, o);
+      if ((tid & 31) >= o) upto += u;
+    }
+    int at = 0;
+    if ((tid & 31) == 31 && upto > 0) at = atomicAdd(&n_list, upto);
+    at = __shfl_sync(FULL_MASK, at, 31) + upto - __popc(first);
+#pragma unroll
+    for (int j = 0; j < AHEAD; ++j) {
+      if ((first >> j) & 1u) {
+        if (at < LIST) list[at] = static_cast<uint16_t>(ahead[j]);
+        ++at;
+      }
+    }
     for (int t = tid + LT * AHEAD; t < len; t += LT) {
       const int rel = tok[t] - base;
       if (count(t, rel)) push(rel);
