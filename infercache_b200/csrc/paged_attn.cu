@@ -69,21 +69,19 @@ int check(const ic_paged_attn_args* a) {
   return IC_OK;
 }
 
-constexpr int ALL_ROWS = 0x7fffffff;
+}  // namespace
 
 // Sessions with at most this many query rows per KV head are the streaming
 // kernel's.  It reads a session's pages once per 16 rows, the tile kernel
 // converts them once per 256 but gives each (session, KV head, 256 rows) to one
 // CTA: below some 20 such CTAs the streaming kernel's even shares win although
 // it does the work several times over.
-int few_rows(const ic_paged_attn_args* a) {
-  const int64_t G = a->num_q_heads / a->num_kv_heads;
-  if (a->head_dim == 256 || a->max_count * G <= 64 || a->num_q_tokens * static_cast<int64_t>(a->num_q_heads) <= 4096)
+int few_rows(const ic_paged_attn_args& a) {
+  const int64_t G = a.num_q_heads / a.num_kv_heads;
+  if (a.head_dim == 256 || a.max_count * G <= 64 || a.num_q_tokens * static_cast<int64_t>(a.num_q_heads) <= 4096)
     return ALL_ROWS;
   return 64;
 }
-
-}  // namespace
 
 int page_map(CUtensorMap* m, const void* codes, int64_t pool_tokens, int heads, int D) {
   static const EncodeTiledFn fn = find_encode();
@@ -143,7 +141,7 @@ extern "C" int ic_paged_attention(const ic_paged_attn_args* a, void* stream) {
   p.G = a->num_q_heads / a->num_kv_heads;
   p.n_pages = static_cast<int32_t>(a->pool_tokens / q8::PAGE);
   p.n_q = a->num_q_tokens;
-  p.few_rows = paged::few_rows(a);
+  p.few_rows = paged::few_rows(*a);
   p.min_share = 16;
   p.sl2 = a->scale * paged::LOG2E;
   cudaStream_t st = static_cast<cudaStream_t>(stream);

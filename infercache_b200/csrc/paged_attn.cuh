@@ -52,6 +52,10 @@ __device__ __forceinline__ int held_tokens(const Params& p, int s) {
 // 16-byte chunk c of line r is stored at chunk c ^ (r % 8).
 int page_map(CUtensorMap* m, const void* codes, int64_t pool_tokens, int heads, int D);
 
+// What Params::few_rows is for a call; ALL_ROWS: everything is the streaming kernel's.
+constexpr int ALL_ROWS = 0x7fffffff;
+int few_rows(const ic_paged_attn_args& a);
+
 int launch_stream(const Params& p, const ic_paged_attn_args& a, cudaStream_t st);
 int launch_tile(const Params& p, const ic_paged_attn_args& a, cudaStream_t st);
 // Rows per tile of the streaming kernel: 8 where they hold a whole session's.

@@ -554,8 +554,8 @@ __global__ void __launch_bounds__(NW * 32, ctas_per_sm(D, NG))
 
     // ---- join the warps, 8 rows at a time ----------------------------------------------
     float* wo = reinterpret_cast<float*>(smem + L::MERGE);
-    float* cx = reinterpret_cast<float*>(smem);  // GROUPED: [8][D] in the ring, which is done, and [8][2] behind it
-    float* cs = cx + 8 * D;
+    float* cx = reinterpret_cast<float*>(smem);  // GROUPED: [ROWS][D] in the ring, which is done, and [ROWS][2] behind it
+    float* cs = cx + ROWS * D;
     const bool whole = seg.p0 == 0 && seg.p1 == seg.pages;
     const int slot = 2 * cta + (pos == pos0 ? 0 : 1);
 #pragma unroll
@@ -591,8 +591,8 @@ __global__ void __launch_bounds__(NW * 32, ctas_per_sm(D, NG))
         }
         const size_t prow = static_cast<size_t>(slot) * ROWS + nt * 8 + row;
         if (GROUPED) {  // this CTA's part, for the cluster to read
-          *reinterpret_cast<float4*>(cx + row * D + d0) = x;
-          if (d0 == 0) *reinterpret_cast<float2*>(cs + row * 2) = make_float2(m, lsum);
+          *reinterpret_cast<float4*>(cx + (nt * 8 + row) * D + d0) = x;
+          if (d0 == 0) *reinterpret_cast<float2*>(cs + (nt * 8 + row) * 2) = make_float2(m, lsum);
         } else if (!whole) {
           *reinterpret_cast<float4*>(part + prow * D + d0) = x;
           if (d0 == 0) *reinterpret_cast<float2*>(part_stat + prow * 2) = make_float2(m, lsum);
@@ -605,31 +605,31 @@ __global__ void __launch_bounds__(NW * 32, ctas_per_sm(D, NG))
       __syncthreads();
     }
     if (GROUPED) {
-      // Every CTA's 8 rows lie in its shared memory; CTA j finishes rows j, j + CL,
+      // Every CTA's rows lie in its shared memory; CTA j finishes rows j, j + CL,
       // ..., a warp each, adding the parts in the CTAs' order.
       cluster_arrive_release();
       cluster_wait_acquire();
-      const int row = rank + warp * CL, r = row0 + row;
-      if (row < 8 && r < rows) {
+      for (int row = rank + warp * CL; row < ROWS && row0 + row < rows; row += NW * CL) {
+        const int r = row0 + row;
         const uint32_t sa = smem_addr(cs + row * 2), xa = smem_addr(cx + row * D);
-        float m = -INFINITY;
-        for (int j = 0; j < CL; ++j) m = fmaxf(m, ld_cluster2(map_shared(sa, j)).x);
+        // lane j holds part j's maximum and sum
+        const float2 ml = lane < CL ? ld_cluster2(map_shared(sa, lane)) : make_float2(-INFINITY, 0.f);
+        const float m = warp_max(ml.x), f = ml.x == -INFINITY ? 0.f : tc::ex2(ml.x - m);
         float lsum = 0.f;
-        for (int j = 0; j < CL; ++j) {
-          const float2 v = ld_cluster2(map_shared(sa, j));
-          lsum = fmaf(v.y, v.x == -INFINITY ? 0.f : tc::ex2(v.x - m), lsum);
-        }
+        for (int j = 0; j < CL; ++j) lsum = fmaf(__shfl_sync(FULL_MASK, ml.y, j), __shfl_sync(FULL_MASK, f, j), lsum);
         const int64_t orow = static_cast<int64_t>(seg.q_begin + r / p.G) * p.Hq + h * p.G + r % p.G;
 #pragma unroll
-        for (int d0 = lane * 4; d0 < D; d0 += 128) {
+        for (int d1 = 0; d1 < D; d1 += 128) {
+          const int d0 = d1 + lane * 4;
           float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
           for (int j = 0; j < CL; ++j) {
-            const float mj = ld_cluster2(map_shared(sa, j)).x;
-            const float f = mj == -INFINITY ? 0.f : tc::ex2(mj - m);
-            const float4 u = ld_cluster4(map_shared(xa + d0 * 4, j));
-            x.x = fmaf(u.x, f, x.x); x.y = fmaf(u.y, f, x.y); x.z = fmaf(u.z, f, x.z); x.w = fmaf(u.w, f, x.w);
+            const float fj = __shfl_sync(FULL_MASK, f, j);
+            if (d0 < D) {
+              const float4 u = ld_cluster4(map_shared(xa + d0 * 4, j));
+              x.x = fmaf(u.x, fj, x.x); x.y = fmaf(u.y, fj, x.y); x.z = fmaf(u.z, fj, x.z); x.w = fmaf(u.w, fj, x.w);
+            }
           }
-          store_row<QT>(static_cast<QT*>(p.out) + orow * D + d0, x, lsum);
+          if (d0 < D) store_row<QT>(static_cast<QT*>(p.out) + orow * D + d0, x, lsum);
         }
         if (lane == 0 && p.lse) p.lse[orow] = lse_of(m, lsum);
       }
@@ -746,10 +746,10 @@ __global__ void __launch_bounds__(JT) join_kernel(const Params p) {
   }
 }
 
-// At most this many groups of 8 rows, whatever the sessions' counts.
-int64_t group_bound(const ic_paged_attn_args& a) {
+// At most this many groups of `rows` rows, whatever the sessions' counts.
+int64_t group_bound(const ic_paged_attn_args& a, int rows) {
   const int64_t G = a.num_q_heads / a.num_kv_heads, n = a.num_q_tokens;
-  return std::min<int64_t>(n * ((G + 7) / 8), n * G / 8 + std::min<int64_t>(a.num_sessions, n)) * a.num_kv_heads;
+  return std::min<int64_t>(n * ((G + rows - 1) / rows), n * G / rows + std::min<int64_t>(a.num_sessions, n)) * a.num_kv_heads;
 }
 // CTAs per group when each group gets a cluster of its own, 0 for shares of the
 // line.  A cluster joins its parts through distributed shared memory, without
@@ -757,11 +757,10 @@ int64_t group_bound(const ic_paged_attn_args& a) {
 // 8 CTAs: so only while all clusters run at once and the table's width leaves a
 // CTA at most MAX_CTA_PAGES pages.
 constexpr int MAX_CTA_PAGES = 96;
-int cluster_size(const ic_paged_attn_args& a, int per_sm) {
-  const int64_t groups = group_bound(a);
-  for (int cl = 8; cl >= 2; cl /= 2)
-    if (groups * cl <= SMS * per_sm) return a.table_width <= MAX_CTA_PAGES * cl ? cl : 0;
-  return 0;
+int cluster_size(const ic_paged_attn_args& a, int rows) {
+  const int64_t groups = group_bound(a, rows);
+  const int64_t cl = std::min<int64_t>(8, SMS * ctas_per_sm(a.head_dim, rows / 8) / groups);
+  return cl >= 2 && a.table_width <= MAX_CTA_PAGES * cl ? static_cast<int>(cl) : 0;
 }
 
 template <typename QT, int D, int CODE, int NG>
@@ -772,29 +771,26 @@ int launch(const Params& p, const ic_paged_attn_args& a, cudaStream_t st) {
   if ((rc = page_map(&mv, a.v, a.pool_tokens, p.H, D)) != IC_OK) return rc;
   Params params = p;
   const int smem = Layout<D, NG>::bytes(p.S);
-  if constexpr (NG == 1) {
-    const int cl = cluster_size(a, ctas_per_sm(D, NG));
-    if (cl > 0) {
-      static PerDeviceLimit grouped_limit;
-      auto kern = stream_kernel<QT, D, CODE, NG, true>;
-      if ((rc = ensure_dynamic_smem(kern, smem, &grouped_limit)) != IC_OK) return rc;
-      params.cluster = cl;
-      cudaLaunchConfig_t cfg = {};
-      cfg.gridDim = dim3(static_cast<unsigned>(group_bound(a) * cl));
-      cfg.blockDim = dim3(NW * 32);
-      cfg.dynamicSmemBytes = smem;
-      cfg.stream = st;
-      cudaLaunchAttribute attr[2];
-      attr[0].id = cudaLaunchAttributeClusterDimension;
-      attr[0].val.clusterDim.x = cl;
-      attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-      attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-      attr[1].val.programmaticStreamSerializationAllowed = 1;
-      cfg.attrs = attr;
-      cfg.numAttrs = 2;
-      cudaLaunchKernelEx(&cfg, kern, mk, mv, params);
-      return launch_status("paged_attention (stream, grouped)");
-    }
+  if (const int cl = p.few_rows == ALL_ROWS ? cluster_size(a, 8 * NG) : 0) {
+    static PerDeviceLimit grouped_limit;
+    auto kern = stream_kernel<QT, D, CODE, NG, true>;
+    if ((rc = ensure_dynamic_smem(kern, smem, &grouped_limit)) != IC_OK) return rc;
+    params.cluster = cl;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(static_cast<unsigned>(group_bound(a, 8 * NG) * cl));
+    cfg.blockDim = dim3(NW * 32);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = cl;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 2;
+    cudaLaunchKernelEx(&cfg, kern, mk, mv, params);
+    return launch_status("paged_attention (stream, grouped)");
   }
   auto kern = stream_kernel<QT, D, CODE, NG, false>;
   static PerDeviceLimit limit;
@@ -833,9 +829,8 @@ int launch_dim(const Params& p, const ic_paged_attn_args& a, cudaStream_t st, bo
 
 int64_t stream_workspace(const ic_paged_attn_args& a) {
   const int rows = stream_rows(static_cast<int64_t>(a.max_count) * (a.num_q_heads / a.num_kv_heads));
-  const int per_sm = ctas_per_sm(a.head_dim, rows / 8);
-  if (rows == 8 && cluster_size(a, per_sm) > 0) return 0;
-  const int64_t ctas = SMS * per_sm;
+  if (few_rows(a) == ALL_ROWS && cluster_size(a, rows) > 0) return 0;
+  const int64_t ctas = SMS * ctas_per_sm(a.head_dim, rows / 8);
   return 2 * ctas * rows * (a.head_dim + 2) * 4 + ctas * static_cast<int64_t>(sizeof(Task));
 }
 
