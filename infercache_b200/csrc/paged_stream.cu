@@ -466,8 +466,6 @@ __global__ void __launch_bounds__(NW * 32, ctas_per_sm(D, NG))
             for (int c = 0; c < W4; ++c) t[x][c] = 0;
           }
         }
-        __syncwarp();  // the page is in registers: its stage takes the next one
-        issue(seg, st, next);
         const bool edge = tok0 + q8::PAGE > lim_all;
         bool over = false;
 #pragma unroll
@@ -526,9 +524,12 @@ __global__ void __launch_bounds__(NW * 32, ctas_per_sm(D, NG))
               Mma<__half>::run(o[nt][2 * c + half], a0, a1, a2, a3, pb[nt][0], pb[nt][1]);
           }
         }
-      } else {
-        issue(seg, st, next);
       }
+      // Not before the products have consumed what was loaded from the page: a load
+      // that is merely issued may still be under way when the next page's copy
+      // begins to land in this stage.
+      __syncwarp();
+      issue(seg, st, next);
       st = wrap(st + 1);
     }
     if (dead) {  // copies in flight land before their buffers are given up (short waits)
