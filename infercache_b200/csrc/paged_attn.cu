@@ -62,7 +62,7 @@ int check(const ic_paged_attn_args* a) {
   // the streaming kernel numbers all groups' pages with 32 bits
   const int64_t G = a->num_q_heads / a->num_kv_heads;
   const int64_t tiles = a->num_q_tokens * G / 8 + a->num_sessions;
-  if (tiles * a->num_kv_heads > 0x7fffffffLL / (a->table_width > 0 ? a->table_width : 1)) {
+  if (tiles * a->num_kv_heads > 0x7fffffffLL / (a->table_width + 32)) {
     set_last_error("paged_attention: query tiles x KV heads x table width exceed 2^31");
     return IC_ERR_UNSUPPORTED;
   }
@@ -142,7 +142,7 @@ extern "C" int ic_paged_attention(const ic_paged_attn_args* a, void* stream) {
   p.n_pages = static_cast<int32_t>(a->pool_tokens / q8::PAGE);
   p.n_q = a->num_q_tokens;
   p.few_rows = paged::few_rows(*a);
-  p.min_share = 16;
+  p.min_share = 32;
   p.sl2 = a->scale * paged::LOG2E;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (p.few_rows != paged::ALL_ROWS && (rc = paged::launch_tile(p, *a, st)) != IC_OK) return rc;

@@ -4,11 +4,21 @@
 //
 // Work.  A session's query rows (its new tokens x the query heads of a KV
 // head) are cut into tiles of 8 or 16 rows; a (session, KV head, tile) is a
-// group, its pages a run of units.  All groups' pages form one line, cut into
-// equal shares, one per CTA, so that ragged lengths and a single long session
-// balance alike.  A CTA walks its share group by group; a group that ends up in
-// several shares leaves partial (max, sum, O) per share, which a second small
-// kernel joins in share order.  Nothing depends on an order of atomics.
+// group, its pages a run of units.  Two ways to deal them out (cluster_size):
+//  * a cluster of 1 to 8 CTAs per group, joined through distributed shared
+//    memory, while the table's width bounds what a CTA gets;
+//  * for wide tables, all groups' pages on one line, OVERHEAD units before each
+//    group's first, cut into equal shares, one per CTA, so that ragged lengths
+//    and a single long session balance alike.  A CTA walks its share group by
+//    group; a group that ends up in several shares leaves partial (max, sum, O)
+//    per share, which a second small kernel joins in share order.
+// Nothing depends on an order of atomics.
+//
+// Measured (B200, 128 dims): 64 sessions of 1k to 8k tokens, 4 KV heads of 7 query
+// heads, 57.8 us: 5.2 TB/s of codes and scales, 80 % of a plain copy's rate; 16
+// of 2k, 2 heads of 8, 12.2 us (clusters of 8); one of 128k, 2 heads of 8, 23.6 us,
+// of which the join is 4; one of 300 tokens, 2 heads of 6, 6.8 us (launch and
+// dependent loads: q, table, scales, pages).
 //
 // Inside a CTA each warp streams its own pages (every 8th of the segment)
 // through a ring of its own: one elected lane issues two TMA box copies per
@@ -47,6 +57,11 @@ namespace {
 
 constexpr int SMS = 148;
 constexpr int NW = 8;                 // warps per CTA
+// What a group costs a CTA besides its pages, in pages: about 2.5 us to begin and
+// to join its warps, against 0.1 us a page.  (Counting pages alone gave one CTA 16
+// groups of one page: 83 sessions of 6 tokens, 4 heads of 16: 98 us, now 25; the 64
+// sessions of up to 8k tokens: 62 us, now 58.)
+constexpr int OVERHEAD = 24;
 constexpr float TINY = 7.8886090522101181e-31f;  // 2^-100
 constexpr float SLACK = 8.f;          // u may pass M by this much
 constexpr float LIFT = 7.f;           // P' = 2^(u - M + LIFT): at most 2^15
@@ -187,8 +202,8 @@ __global__ void __launch_bounds__(NW * 32, ctas_per_sm(D, NG))
     tok = query_tokens(p, x, begin);
     len = held_tokens(p, x);
     const int rows = tok * p.G;
-    const int pages = GROUPED ? 1 : max(1, (len + q8::PAGE - 1) / q8::PAGE);
-    return rows <= p.few_rows ? (rows + ROWS - 1) / ROWS * p.H * pages : 0;
+    const int units = GROUPED ? 1 : OVERHEAD + max(1, (len + q8::PAGE - 1) / q8::PAGE);
+    return rows <= p.few_rows ? (rows + ROWS - 1) / ROWS * p.H * units : 0;
   };
   if (lanes) {
     if (lane < p.S) l_upto = units_of(lane, l_begin, l_tok, l_len);
@@ -240,10 +255,11 @@ __global__ void __launch_bounds__(NW * 32, ctas_per_sm(D, NG))
   bool dead = false;     // a wait gave up: nothing more is loaded
   int st = 0;            // stage of the next page to be consumed
 
-  // A segment: session s, KV head h, row tile, pages p0 .. p1 of the group; this
-  // warp's are p0 + gw + stride * i, i < mine.
+  // A segment: session s, KV head h, row tile, pages p0 .. p1 of the group (none
+  // when the share ends before the group's first page); this warp's are p0 + gw +
+  // stride * i, i < mine.
   struct Seg {
-    int s, h, q_begin, n_tok, len, row0, pages, p0, p1, mine;
+    int s, h, q_begin, n_tok, len, row0, pages, p0, p1, mine, end;  // end: of the group, on the line
   };
   const auto find = [&](int pos, int from) {
     Seg g;
@@ -268,9 +284,11 @@ __global__ void __launch_bounds__(NW * 32, ctas_per_sm(D, NG))
     }
     g.pages = max(1, (g.len + q8::PAGE - 1) / q8::PAGE);
     const uint32_t tiles = static_cast<uint32_t>(g.n_tok * p.G + ROWS - 1) / ROWS, at = pos - before;
-    const uint32_t gi = GROUPED ? at : at / static_cast<uint32_t>(g.pages), hh = tiles == 1 ? gi : gi / tiles;
-    g.p0 = GROUPED ? 0 : at - gi * g.pages;
-    g.p1 = GROUPED ? g.pages : min(g.pages, g.p0 + (end - pos));
+    const uint32_t units = OVERHEAD + g.pages, gi = GROUPED ? at : at / units, hh = tiles == 1 ? gi : gi / tiles;
+    const int off = at - gi * units - OVERHEAD;  // units before the first page are negative
+    g.p0 = GROUPED ? 0 : max(off, 0);
+    g.p1 = GROUPED ? g.pages : max(0, min(g.pages, off + (end - pos)));
+    g.end = pos - off + g.pages;
     g.h = hh;
     g.row0 = (gi - hh * tiles) * ROWS;
     g.mine = g.p1 - g.p0 > gw ? static_cast<uint32_t>(g.p1 - g.p0 - gw + stride - 1) / static_cast<uint32_t>(stride) : 0;
@@ -537,7 +555,7 @@ __global__ void __launch_bounds__(NW * 32, ctas_per_sm(D, NG))
     }
 
     // ---- the next segment's first pages are on their way while this one is joined ------
-    const int next_pos = pos + seg.p1 - seg.p0;
+    const int next_pos = min(seg.end, end);
     const bool more = !GROUPED && next_pos < end;
     Seg nseg;
     int nid = -1;
@@ -594,7 +612,7 @@ __global__ void __launch_bounds__(NW * 32, ctas_per_sm(D, NG))
         if (GROUPED) {  // this CTA's part, for the cluster to read
           *reinterpret_cast<float4*>(cx + (nt * 8 + row) * D + d0) = x;
           if (d0 == 0) *reinterpret_cast<float2*>(cs + (nt * 8 + row) * 2) = make_float2(m, lsum);
-        } else if (!whole) {
+        } else if (!whole) {  // (a segment without pages stores a partial that nobody reads)
           *reinterpret_cast<float4*>(part + prow * D + d0) = x;
           if (d0 == 0) *reinterpret_cast<float2*>(part_stat + prow * 2) = make_float2(m, lsum);
         } else if (r < rows) {
@@ -638,13 +656,13 @@ __global__ void __launch_bounds__(NW * 32, ctas_per_sm(D, NG))
       cluster_wait_acquire();
       break;
     }
-    if (tid == 0 && seg.p0 == 0 && seg.p1 < seg.pages) {  // this CTA holds the group's first page, not its last
+    if (tid == 0 && seg.p0 == 0 && seg.p1 > 0 && seg.p1 < seg.pages) {  // the group's first page, not its last
       Task t;
       t.valid = 1;
       t.s = s;
       t.h = h;
       t.tile = row0 / ROWS;
-      t.last_cta = (pos + seg.pages - 1) / share;
+      t.last_cta = (seg.end - 1) / share;
       t.first_slot = slot;
       tasks[cta] = t;
     }
@@ -755,13 +773,14 @@ int64_t group_bound(const ic_paged_attn_args& a, int rows) {
 // CTAs per group when each group gets a cluster of its own, 0 for shares of the
 // line.  A cluster joins its parts through distributed shared memory, without
 // the 3 to 4 us of a second kernel, but a group is then split over no more than
-// 8 CTAs: so only while all clusters run at once and the table's width leaves a
-// CTA at most MAX_CTA_PAGES pages.
+// 8 CTAs, or left whole when there are many groups: so only while the table's
+// width leaves a CTA at most MAX_CTA_PAGES pages.  (33 sessions x 19 tokens x 8
+// heads of 8 at 256 dims: shares of the line 859 us, a CTA per group 264.)
 constexpr int MAX_CTA_PAGES = 96;
 int cluster_size(const ic_paged_attn_args& a, int rows) {
   const int64_t groups = group_bound(a, rows);
-  const int64_t cl = std::min<int64_t>(8, SMS * ctas_per_sm(a.head_dim, rows / 8) / groups);
-  return cl >= 2 && a.table_width <= MAX_CTA_PAGES * cl ? static_cast<int>(cl) : 0;
+  const int64_t cl = std::max<int64_t>(1, std::min<int64_t>(8, SMS * ctas_per_sm(a.head_dim, rows / 8) / groups));
+  return a.table_width <= MAX_CTA_PAGES * cl && groups * cl <= 0x7fffffff ? static_cast<int>(cl) : 0;
 }
 
 template <typename QT, int D, int CODE, int NG>
