@@ -19,7 +19,7 @@
 namespace ic {
 namespace {
 
-constexpr int WARPS = 8;  // warps per CTA (write)
+constexpr int WARPS = 4;  // warps per CTA (write)
 
 struct Range {
   const int32_t* slots;
@@ -139,6 +139,14 @@ __device__ __forceinline__ void store_codes(uint32_t* dst, const uint32_t* o) {
     *dst = o[0];
 }
 
+// A page's source rows pass through CHUNK vectors per lane twice, for the
+// maximum and for the codes; the second reading hits the cache and a run of one
+// or two tokens needs none.  Holding the whole page instead (8 to 32 vectors)
+// is 3 % faster for long prompts (write-out of 16 x 2k tokens: 599 against
+// 617 us) but leaves a third of the warps: 78 against 65 us for one token of
+// 149 sessions in 28 layers, 29 against 12 us for 24 tokens of each in one.
+constexpr int CHUNK = 4;
+
 // `cnt` tokens, source rows src + t * stride (elements), into slots off ..
 // off + cnt - 1 of the page at `page` (16 rows of D codes).
 template <typename T, int D, int CODE>
@@ -147,26 +155,34 @@ __device__ __forceinline__ void write_run(const T* src, int64_t stride, int cnt,
   constexpr int E = VE<T>, W = E / 4;         // elements and code words per vector
   constexpr int VR = D / E;                   // vectors per row
   constexpr int NV = q8::PAGE * VR / 32;      // vectors per lane for a whole page
+  constexpr int CH = NV < CHUNK ? NV : CHUNK; // of which so many are held at a time
   const T* type = nullptr;
-  uint4 raw[NV];
+  const int chunks = (cnt * VR + 32 * CH - 1) / (32 * CH);
+  uint4 raw[CH];
+  const auto load_chunk = [&](int c) {
 #pragma unroll
-  for (int j = 0; j < NV; ++j) {
-    const int it = lane + 32 * j, t = it / VR;
-    raw[j] = make_uint4(0, 0, 0, 0);
-    if (t < cnt) raw[j] = reinterpret_cast<const uint4*>(src + t * stride)[it % VR];
-  }
+    for (int j = 0; j < CH; ++j) {
+      const int it = lane + 32 * (c * CH + j), t = it / VR;
+      raw[j] = make_uint4(0, 0, 0, 0);
+      if (t < cnt) raw[j] = reinterpret_cast<const uint4*>(src + t * stride)[it % VR];
+    }
+  };
   const float held = off > 0 ? *scale_p : 0.f;
   uint32_t m = 0;
+#pragma unroll 1
+  for (int c = chunks - 1; c >= 0; --c) {     // ends with chunk 0 in registers
+    load_chunk(c);
 #pragma unroll
-  for (int j = 0; j < NV; ++j) m = max_bits<T>(m, raw[j]);
+    for (int j = 0; j < CH; ++j) m = max_bits<T>(m, raw[j]);
+  }
   uint32_t amax = warp_max_bits(m, type);
   bool plain = amax < 0x7f800000u;            // every value finite
   if (!plain) {
     amax = 0;
-#pragma unroll
-    for (int j = 0; j < NV; ++j) {
+#pragma unroll 1
+    for (int it = lane; it < cnt * VR; it += 32) {
       float x[E];
-      vec_floats(raw[j], x, type);
+      vec_floats(reinterpret_cast<const uint4*>(src + it / VR * stride)[it % VR], x, type);
 #pragma unroll
       for (int i = 0; i < E; ++i) {
         const uint32_t b = __float_as_uint(x[i]) & 0x7fffffffu;
@@ -195,30 +211,36 @@ __device__ __forceinline__ void write_run(const T* src, int64_t stride, int cnt,
     }
   }
   uint32_t* dst = reinterpret_cast<uint32_t*>(page + off * D);
-  if (plain && sizeof(T) == 2 && std::is_same<T, __half>::value && e >= -15 && e <= 24) {
+  if (plain) {
+    const bool in_half = std::is_same<T, __half>::value && e >= -15 && e <= 24;
     const __half2 unit = __float2half2_rn(q8::two_to(-e));
+#pragma unroll 1
+    for (int c = 0;;) {
+      if (in_half) {
 #pragma unroll
-    for (int j = 0; j < NV; ++j) {
-      const int it = lane + 32 * j;
-      uint32_t o[2];
-      encode_half<CODE>(raw[j], unit, o);
-      if (it / VR < cnt) store_codes<W>(dst + it * W, o);
-    }
-  } else if (plain) {
+        for (int j = 0; j < CH; ++j) {
+          const int it = lane + 32 * (c * CH + j);
+          uint32_t o[2];
+          encode_half<CODE>(raw[j], unit, o);
+          if (it / VR < cnt) store_codes<W>(dst + it * W, o);
+        }
+      } else {
 #pragma unroll
-    for (int j = 0; j < NV; ++j) {
-      const int it = lane + 32 * j;
-      uint32_t o[W];
-      encode_vec<CODE>(raw[j], e, o, type);
-      if (it / VR < cnt) store_codes<W>(dst + it * W, o);
+        for (int j = 0; j < CH; ++j) {
+          const int it = lane + 32 * (c * CH + j);
+          uint32_t o[W];
+          encode_vec<CODE>(raw[j], e, o, type);
+          if (it / VR < cnt) store_codes<W>(dst + it * W, o);
+        }
+      }
+      if (++c >= chunks) break;
+      load_chunk(c);                          // again, from the cache
     }
   } else {
     const float unit = q8::two_to(-e);
 #pragma unroll 1
-    for (int j = 0; j < NV; ++j) {
-      const int it = lane + 32 * j, t = it / VR;
-      if (t >= cnt) break;
-      const uint4 u = reinterpret_cast<const uint4*>(src + t * stride)[it % VR];
+    for (int it = lane; it < cnt * VR; it += 32) {
+      const uint4 u = reinterpret_cast<const uint4*>(src + it / VR * stride)[it % VR];
       float x[E];
       vec_floats(u, x, type);
 #pragma unroll
@@ -448,13 +470,13 @@ extern "C" int ic_page_write_q8(const ic_page_q8_args* a, void* stream) {
   if (planes == 0) return IC_OK;
   Batch b = {};
   fill_batch(a, b);
-  // Slots form: a warp looks after one token's run when that still leaves few
-  // warps (a decode tick: every run is one token and all run side by side),
-  // else after the runs that begin among 16 tokens, so that a prompt's warps
-  // have a page each instead of fifteen in sixteen finding nothing to do.
+  // Slots form: a warp looks after the runs that begin among `window` tokens.
+  // One while that leaves few warps (a decode tick: every run is one token and
+  // all run side by side); with many, 4 and then 16, so that a prompt's warps
+  // have a page each instead of most of them finding nothing to do.
   int64_t tokens = 0;
   for (int i = 0; i < a->count; ++i) tokens += a->rows[i].n_tokens;
-  b.window = tokens * planes <= 16384 ? 1 : 16;
+  b.window = tokens * planes <= 8192 ? 1 : tokens * planes <= 65536 ? 4 : 16;
   for (int i = 0; i < a->count; ++i) {
     const ic_page_q8_rows& r = a->rows[i];
     const int64_t items = r.n_tokens == 0 ? 0
