@@ -16,8 +16,8 @@
 //
 // Measured (B200, 128 dims): 64 sessions of 1k to 8k tokens, 4 KV heads of 7 query
 // heads, 57.8 us: 5.2 TB/s of codes and scales, 80 % of a plain copy's rate; 16
-// of 2k, 2 heads of 8, 12.2 us (clusters of 8); one of 128k, 2 heads of 8, 23.6 us,
-// of which the join is 4; one of 300 tokens, 2 heads of 6, 6.8 us (launch and
+// of 2k, 2 heads of 8, 12.2 us (clusters of 8); one of 128k, as many heads, 23.6 us,
+// of which the join is 4; one of 300 tokens 6.8 us (launch and
 // dependent loads: q, table, scales, pages).
 //
 // Inside a CTA each warp streams its own pages (every 8th of the segment)
