@@ -556,6 +556,9 @@ int ic_graph_select(const ic_graph_select_args* a, void* stream);
  * are powers of two between 2^-60 and 2^60: the smallest 2^e with
  * max |x| <= 448 * 2^e (IC_E4M3) or 127 * 2^e (IC_I8) over the page's
  * values, so code * scale is exact in 32 bits and scaling adds no rounding.
+ * A pool filled by other means keeps to that: positive scales, and no NaN code
+ * (IC_E4M3 0x7f, 0xff) in a session's rows, where it may reach every query of
+ * the session.
  * ====================================================================== */
 
 /* ---- Block tables and slot maps from request lengths ----------------------

@@ -59,7 +59,8 @@ int check(const ic_paged_attn_args* a) {
     set_last_error("paged_attention: at most 4096 sessions");
     return IC_ERR_UNSUPPORTED;
   }
-  // the streaming kernel numbers all groups' pages with 32 bits
+  // the streaming kernel numbers all groups' pages, and its overhead for each
+  // group, with 32 bits
   const int64_t G = a->num_q_heads / a->num_kv_heads;
   const int64_t tiles = a->num_q_tokens * G / 8 + a->num_sessions;
   if (tiles * a->num_kv_heads > 0x7fffffffLL / (a->table_width + 32)) {

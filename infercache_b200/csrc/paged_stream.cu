@@ -205,12 +205,17 @@ __global__ void __launch_bounds__(NW * 32, ctas_per_sm(D, NG))
     const int units = GROUPED ? 1 : OVERHEAD + max(1, (len + q8::PAGE - 1) / q8::PAGE);
     return rows <= p.few_rows ? (rows + ROWS - 1) / ROWS * p.H * units : 0;
   };
+  // One session's units fit 31 bits, and so do all while q_start ascends; where it
+  // does not, the sums stop at 2^31 - 1 and every index still stays in its range.
+  const auto add = [](int x, int y) {
+    return static_cast<int>(min(static_cast<uint32_t>(x) + static_cast<uint32_t>(y), 0x7fffffffu));
+  };
   if (lanes) {
     if (lane < p.S) l_upto = units_of(lane, l_begin, l_tok, l_len);
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const int u = __shfl_up_sync(FULL_MASK, l_upto, o);
-      if (lane >= o) l_upto += u;
+      if (lane >= o) l_upto = add(l_upto, u);
     }
     total = __shfl_sync(FULL_MASK, l_upto, 31);
     __syncthreads();  // the barriers are initialised
@@ -223,17 +228,17 @@ __global__ void __launch_bounds__(NW * 32, ctas_per_sm(D, NG))
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
         const int u = __shfl_up_sync(FULL_MASK, w, o);
-        if (lane >= o) w += u;
+        if (lane >= o) w = add(w, u);
       }
       if (lane == 31) scan[warp] = w;
       __syncthreads();
       int before = carry;
 #pragma unroll
       for (int i = 0; i < NW; ++i) {
-        if (i < warp) before += scan[i];
-        carry += scan[i];
+        if (i < warp) before = add(before, scan[i]);
+        carry = add(carry, scan[i]);
       }
-      if (s < p.S) prefix[s + 1] = before + w;
+      if (s < p.S) prefix[s + 1] = add(before, w);
       __syncthreads();
     }
     total = prefix[p.S];
@@ -255,9 +260,8 @@ __global__ void __launch_bounds__(NW * 32, ctas_per_sm(D, NG))
   bool dead = false;     // a wait gave up: nothing more is loaded
   int st = 0;            // stage of the next page to be consumed
 
-  // A segment: session s, KV head h, row tile, pages p0 .. p1 of the group (none
-  // when the share ends before the group's first page); this warp's are p0 + gw +
-  // stride * i, i < mine.
+  // A segment: session s, KV head h, row tile, pages p0 .. p1 of the group (at
+  // least one); this warp's are p0 + gw + stride * i, i < mine.
   struct Seg {
     int s, h, q_begin, n_tok, len, row0, pages, p0, p1, mine, end;  // end: of the group, on the line
   };
@@ -287,8 +291,8 @@ __global__ void __launch_bounds__(NW * 32, ctas_per_sm(D, NG))
     const uint32_t units = OVERHEAD + g.pages, gi = GROUPED ? at : at / units, hh = tiles == 1 ? gi : gi / tiles;
     const int off = at - gi * units - OVERHEAD;  // units before the first page are negative
     g.p0 = GROUPED ? 0 : max(off, 0);
-    g.p1 = GROUPED ? g.pages : max(0, min(g.pages, off + (end - pos)));
-    g.end = pos - off + g.pages;
+    g.p1 = GROUPED ? g.pages : min(g.pages, off + (end - pos));
+    g.end = static_cast<int>(min(static_cast<uint32_t>(pos - off) + g.pages, 0x7fffffffu));
     g.h = hh;
     g.row0 = (gi - hh * tiles) * ROWS;
     g.mine = g.p1 - g.p0 > gw ? static_cast<uint32_t>(g.p1 - g.p0 - gw + stride - 1) / static_cast<uint32_t>(stride) : 0;
@@ -555,8 +559,9 @@ __global__ void __launch_bounds__(NW * 32, ctas_per_sm(D, NG))
     }
 
     // ---- the next segment's first pages are on their way while this one is joined ------
-    const int next_pos = min(seg.end, end);
-    const bool more = !GROUPED && next_pos < end;
+    // (a share that ends before the next group's first page has no part of it)
+    const int next_pos = seg.end;
+    const bool more = !GROUPED && next_pos < end - OVERHEAD;
     Seg nseg;
     int nid = -1;
     if (more) {
@@ -612,7 +617,7 @@ __global__ void __launch_bounds__(NW * 32, ctas_per_sm(D, NG))
         if (GROUPED) {  // this CTA's part, for the cluster to read
           *reinterpret_cast<float4*>(cx + (nt * 8 + row) * D + d0) = x;
           if (d0 == 0) *reinterpret_cast<float2*>(cs + (nt * 8 + row) * 2) = make_float2(m, lsum);
-        } else if (!whole) {  // (a segment without pages stores a partial that nobody reads)
+        } else if (!whole) {
           *reinterpret_cast<float4*>(part + prow * D + d0) = x;
           if (d0 == 0) *reinterpret_cast<float2*>(part_stat + prow * 2) = make_float2(m, lsum);
         } else if (r < rows) {
@@ -656,13 +661,13 @@ __global__ void __launch_bounds__(NW * 32, ctas_per_sm(D, NG))
       cluster_wait_acquire();
       break;
     }
-    if (tid == 0 && seg.p0 == 0 && seg.p1 > 0 && seg.p1 < seg.pages) {  // the group's first page, not its last
+    if (tid == 0 && seg.p0 == 0 && seg.p1 < seg.pages) {  // this CTA holds the group's first page, not its last
       Task t;
       t.valid = 1;
       t.s = s;
       t.h = h;
       t.tile = row0 / ROWS;
-      t.last_cta = (seg.end - 1) / share;
+      t.last_cta = (min(seg.end, total) - 1) / share;
       t.first_slot = slot;
       tasks[cta] = t;
     }
