@@ -44,8 +44,8 @@ class PagedBatch:
         if not pool.quantised:
             raise ValueError(f"PagedBatch needs an 8-bit pool (float8_e4m3fn or int8), got {pool.cfg.dtype}")
         width = pool.cfg.max_pages_per_session if max_pages_per_session is None else int(max_pages_per_session)
-        if max_sessions < 1 or width < 1:
-            raise ValueError("max_sessions and max_pages_per_session must be positive")
+        if not 1 <= max_sessions <= 4096 or width < 1:  # paged_attention's limit
+            raise ValueError("max_sessions must be in [1, 4096] and max_pages_per_session positive")
         ids = list(range(pool.cfg.n_pages)) if pages is None else [int(p) for p in pages]
         if len(set(ids)) != len(ids) or any(not 0 <= p < pool.cfg.n_pages for p in ids):
             raise ValueError(f"pages must be distinct ids in [0, {pool.cfg.n_pages})")
@@ -75,6 +75,8 @@ class PagedBatch:
         """Take ``counts[s]`` (>= 0) new tokens for every session: pages, slots
         and positions (``page_plan``).  Counts on the host give ``total`` and
         ``max_count`` themselves; device counts need ``total``, their sum.
+        A session that finds no pages keeps its length, and attend() gives its
+        tokens' rows of that tick no meaning (check_device_status reports it).
         Without ``commit`` the lengths stay as they were until ``commit_plan``,
         and the next ``extend`` or ``release`` drops the plan."""
         if not (isinstance(counts, torch.Tensor) and counts.is_cuda):

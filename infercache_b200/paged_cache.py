@@ -144,7 +144,11 @@ class PagePool:
                     layer_end=layer_end, buf_dtype=_lib.dtype_code(dtype)))
 
     def _q8_source(self, k: torch.Tensor, v: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
-        """k, v on the device, in one floating dtype (k's), rows aligned for the kernel."""
+        """k, v [L', H, T, D] on the device, in one floating dtype (k's), rows aligned for the kernel."""
+        c = self.cfg
+        if k.dim() != 4 or k.shape != v.shape or (k.shape[1], k.shape[3]) != (c.n_heads, c.head_dim):
+            raise ValueError(f"k and v must be [layers, {c.n_heads}, tokens, {c.head_dim}], got {tuple(k.shape)} and "
+                             f"{tuple(v.shape)}")
         k = k.to(self.device)
         v = v.to(self.device, k.dtype)
         if k.stride() != v.stride() or not rows16(k) or not rows16(v):
@@ -240,6 +244,8 @@ class PagePool:
                 if k.shape[2] == 0:
                     continue
                 k, v = self._q8_source(k, v)
+                if k.shape[0] != self.cfg.n_layers:
+                    raise ValueError(f"write_rows_many writes all {self.cfg.n_layers} layers, got {k.shape[0]}")
                 pid = self._page_ids(page_ids)
                 keep.append((pid, k, v))
                 by_dtype.setdefault(k.dtype, []).append(self._q8_rows(pid, len(page_ids), start, k, v))

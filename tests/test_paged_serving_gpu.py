@@ -326,6 +326,44 @@ def test_attention_whatever_the_table_holds(S, G, D):
     check_attention(attention_inputs(S + G + 1, lens, counts, 2, G, D, torch.int8, torch.bfloat16), max_count=1)
 
 
+@pytest.mark.parametrize("seed", range(4))
+@pytest.mark.parametrize("S,G,D", [(5, 1, 64), (40, 5, 128), (40, 12, 128), (24, 3, 256), (150, 16, 64), (9, 16, 256)])
+def test_attention_wide_tables_share_the_line(seed, S, G, D):
+    """Tables too wide for a cluster per group: shares of one line that begin and
+    end anywhere, in a group's pages and in what it costs besides."""
+    g = torch.Generator().manual_seed(seed)
+    lens = [[0, 1, 16, 17, 300, 700, 2500, 4100][i] for i in torch.randint(0, 8, (S,), generator=g).tolist()]
+    counts = [min(n, c) for n, c in zip(lens, torch.randint(0, 4 if G < 12 else 2, (S,), generator=g).tolist())]
+    if not sum(counts):
+        lens[0] = counts[0] = 1
+    q, k, v, ks, vs, table, n, start = attention_inputs(seed, lens, counts, 2, G, D, CODES[seed % 2],
+                                                        [torch.float16, torch.bfloat16][seed % 2])
+    wide = torch.full((S, 900), -1, dtype=torch.int32, device="cuda")
+    wide[:, :table.shape[1]] = table
+    out, lse, status = check_attention((q, k, v, ks, vs, wide, n, start), max_count=max(counts))
+    assert status == 0
+
+
+def test_two_calls_at_once_keep_apart():
+    """Calls on two streams, whose workspaces and outputs are their own."""
+    from infercache_b200.paged_ops import paged_attention
+    calls = []
+    for seed in (1, 2):
+        q, k, v, ks, vs, table, n, start = attention_inputs(seed, [30000, 5000, 17], [2, 1, 1], 2, 4, 128, torch.int8, torch.float16)
+        calls.append((q, k, v, ks, vs, table, n, start))
+    want = [paged_attention(*c, max_count=2) for c in calls]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in calls]
+    got = [[], []]
+    for _ in range(20):
+        for i, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                got[i].append(paged_attention(*calls[i], max_count=2))
+    torch.cuda.synchronize()
+    for w, outs in zip(want, got):
+        assert all(torch.equal(w, o) for o in outs)
+
+
 @pytest.mark.parametrize("codes", CODES)
 def test_attention_scales_far_apart(codes):
     """Page scales over 2^+-20 for V, scores of hundreds, q at bf16's extremes."""
@@ -633,6 +671,31 @@ def test_pool_refusals():
                  lambda: b.attend(0, x.cpu()), lambda: b.attend(0, x, out=x.float()), lambda: b.gather(3, 1)):
         with pytest.raises(ValueError):
             call()
+
+
+def test_pool_refuses_rows_of_another_shape():
+    """Rows that the pool does not have would be read past their end."""
+    pool = make_pool(torch.int8)
+    good = torch.zeros(2, 2, 5, 64, device="cuda").half()
+    for bad in (good[:, :1], good[..., :32], good[0]):
+        with pytest.raises(ValueError):
+            pool.write_rows([3], 0, bad, bad)
+    with pytest.raises(ValueError):
+        pool.write_rows([3], 0, good, good[:, :, :4])
+    with pytest.raises(ValueError):
+        pool.write_rows_many([([3], 0, good[:1], good[:1])])
+    with pytest.raises(_lib_error()):
+        pool.write_rows([3], 0, good, good, layer_begin=1)
+    with pytest.raises(_lib_error()):
+        pool.write_rows([3], 12, good, good)
+    from infercache_b200 import PagedBatch
+    with pytest.raises(ValueError):
+        PagedBatch(pool, 4097)
+
+
+def _lib_error():
+    from infercache_b200 import _lib
+    return _lib.InferCacheError
 
 
 # ---- a run of them together ---------------------------------------------------------------
