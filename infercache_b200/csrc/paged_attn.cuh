@@ -58,13 +58,16 @@ int few_rows(const ic_paged_attn_args& a);
 
 int launch_stream(const Params& p, const ic_paged_attn_args& a, cudaStream_t st);
 int launch_tile(const Params& p, const ic_paged_attn_args& a, cudaStream_t st);
-// Rows per tile of the streaming kernel, 8 or 16.  A tile of 16 costs 1.4 to 2.5
-// times one of 8 (its registers leave half the warps), so it pays where it halves
-// the number of tiles: not up to 8 rows a session, nor for 17 to 24, which make
-// three tiles or two.  Drafts of up to 24 rows at 64 dims (24 sessions of up to 4k
-// tokens): 16.7 against 18.7 us; 24 rows of 64 sessions of 8k at 128 dims: 146
-// against 164; but 16 rows of those: 112 against 99.
-inline int stream_rows(int64_t max_rows) { return max_rows <= 8 || (max_rows > 16 && max_rows <= 24) ? 8 : 16; }
+// Rows per tile of the streaming kernel, 8 or 16.  16 read the pages half as
+// often but cost registers, hence warps, so they pay where they halve the number
+// of tiles: not up to 8 rows a session, nor, up to 128 dims, for 17 to 24, which
+// make three tiles or two.  Measured with 8 and with 16: 24 sessions x up to 4k
+// tokens x 2 heads, 24 rows, 128 dims 22.8 / 24.8 us, 24 x 1400 x 4 heads 19.2 /
+// 25.2 (64 dims 15.5 / 18.4, but 64 sessions of 8k 102 / 90); at 256 dims 24 rows
+// of 64 sessions of 8k 296 / 253; 16 rows of those at 128 dims 112 / 92.
+inline int stream_rows(int64_t max_rows, int head_dim) {
+  return max_rows <= 8 || (max_rows > 16 && max_rows <= 24 && head_dim <= 128) ? 8 : 16;
+}
 int64_t stream_workspace(const ic_paged_attn_args& a);  // bytes, 0 when the call needs none
 
 }  // namespace paged

@@ -66,26 +66,31 @@ constexpr float TINY = 7.8886090522101181e-31f;  // 2^-100
 constexpr float SLACK = 8.f;          // u may pass M by this much
 constexpr float LIFT = 7.f;           // P' = 2^(u - M + LIFT): at most 2^15
 
-// CTAs per SM: two where 128 registers a thread hold q and O without spills.
+// CTAs per SM: two where 128 registers a thread hold O and the rest with hardly a
+// spill.  With 16 rows of 128 dims that is the cluster form (52 bytes of spills;
+// 83 sessions of 12 rows, 4 heads, 80 keys: 18.2 us, one CTA per SM 23.1); shares
+// of the line would spill 228 bytes (3 sessions of up to 29k: 26 us, one CTA 20).
 // Ring stages per warp: what their shared memory leaves beside the merge rows.
-__host__ __device__ constexpr int ctas_per_sm(int D, int NG) { return D * NG > 128 ? 1 : 2; }
-__host__ __device__ constexpr int stages(int D, int NG) { return D == 256 ? 2 : D == 64 ? 5 : NG == 2 ? 5 : 2; }
+__host__ __device__ constexpr int ctas_per_sm(int D, int NG, bool grouped) { return D * NG > (grouped ? 256 : 128) || D == 256 ? 1 : 2; }
+__host__ __device__ constexpr int stages(int D, int NG, bool grouped) { return D == 64 ? 5 : ctas_per_sm(D, NG, grouped) == 1 && D == 128 ? 5 : 2; }
 
 struct Task {  // the group that continues past a CTA's share, when it begins there
   int32_t valid, s, h, tile, last_cta, first_slot;
 };
 
-template <int D, int NG>
+template <int D, int NG, bool GROUPED>
 struct Layout {
   static constexpr int PAGE_B = 16 * D;                      // codes of a page of one head
-  static constexpr int ST = stages(D, NG);
+  static constexpr int ST = stages(D, NG, GROUPED);
   static constexpr int RING = NW * ST * 2 * PAGE_B;
   static constexpr int ROWS = 8 * NG;
   static constexpr int PITCH = D + 4;                        // floats per row of a warp's O
   static constexpr int MERGE = RING;                         // 8 rows of every warp's O
   static constexpr int BARS = MERGE + NW * 8 * PITCH * 4;
   static constexpr int STAT = BARS + NW * ST * 8;            // M, l per warp and row
-  static constexpr int SCAN = STAT + NW * ROWS * 8;
+  static constexpr int QS = STAT + NW * ROWS * 8;            // NG = 2: q as B operands, 16 bytes per lane
+  static constexpr int QB = QS + (NG == 2 ? NG * D * 16 : 0);  // and its rows' scales
+  static constexpr int SCAN = QB + ROWS * 4;
   static constexpr int PREFIX = SCAN + 64;
   static int bytes(int S) { return PREFIX + (S + 1) * 4 + 1024; }  // + alignment
 };
@@ -170,15 +175,22 @@ __device__ __forceinline__ float lse_of(float m, float l) {
 
 // GROUPED: one cluster of CTAs per group instead of shares of the line.
 template <typename QT, int D, int CODE, int NG, bool GROUPED>
-__global__ void __launch_bounds__(NW * 32, ctas_per_sm(D, NG))
+__global__ void __launch_bounds__(NW * 32, ctas_per_sm(D, NG, GROUPED))
     stream_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv, const Params p) {
-  using L = Layout<D, NG>;
+  using L = Layout<D, NG, GROUPED>;
   constexpr int ST = L::ST, ROWS = L::ROWS, MT = D / 16, NC = D / 64, W4 = D / 32;
   constexpr bool SCALE_Q = std::is_same<QT, __nv_bfloat16>::value;
   extern __shared__ unsigned char smem_raw[];
   unsigned char* smem = smem_raw + ((1024 - (smem_addr(smem_raw) & 1023)) & 1023);
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::BARS);
   float* stat = reinterpret_cast<float*>(smem + L::STAT);     // [NW][ROWS][2]
+  // Tiles of 16 rows: q stays in shared memory for all warps, which leaves its
+  // registers to O (in registers: 64 sessions of 8k at 256 dims 155 us instead of
+  // 123, with 300 bytes of spills); warp nt lays out n-tile nt.
+  constexpr bool Q_SHARED = NG == 2;
+  uint4* qs = reinterpret_cast<uint4*>(smem + L::QS);         // [NG][NC * 2][32]
+  const uint32_t qs_lane = smem_addr(smem + L::QS) + (threadIdx.x & 31) * 16;
+  float* q_back = reinterpret_cast<float*>(smem + L::QB);     // [ROWS]
   int32_t* scan = reinterpret_cast<int32_t*>(smem + L::SCAN);
   int32_t* prefix = reinterpret_cast<int32_t*>(smem + L::PREFIX);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -243,7 +255,7 @@ __global__ void __launch_bounds__(NW * 32, ctas_per_sm(D, NG))
     }
     total = prefix[p.S];
   }
-  constexpr uint32_t CTAS = SMS * ctas_per_sm(D, NG);
+  constexpr uint32_t CTAS = SMS * ctas_per_sm(D, NG, false);
   const int share = GROUPED ? 1 : max(static_cast<int>((static_cast<uint32_t>(total) + CTAS - 1) / CTAS), p.min_share);
   const int cta = GROUPED ? blockIdx.x / CL : blockIdx.x;
   const int64_t pos0 = static_cast<int64_t>(cta) * share;
@@ -354,11 +366,13 @@ __global__ void __launch_bounds__(NW * 32, ctas_per_sm(D, NG))
     if (mine > 32) id_n = fetch_id(seg, 32);
 
     // ---- q as the B operand; head rows past the session's are zero ---------------
-    uint32_t qb[NG][NC * 4][2];
+    uint32_t qb[Q_SHARED ? 1 : NG][NC * 4][2];
     float qmul[NG][2];
     int lim[NG][2];      // keys that rows 2 tq, 2 tq + 1 of each n-tile see
 #pragma unroll
-    for (int nt = 0; nt < NG; ++nt) {
+    for (int n = 0; n < (Q_SHARED ? 1 : NG); ++n) {
+      const int nt = Q_SHARED ? warp : n;
+      if (Q_SHARED && warp >= NG) break;
       const int r = row0 + nt * 8 + g;
       const bool ok = r < rows;
       const QT* src = static_cast<const QT*>(p.q);
@@ -393,13 +407,27 @@ __global__ void __launch_bounds__(NW * 32, ctas_per_sm(D, NG))
         q_pairs(va[c], vb[c], f, o, static_cast<QT*>(nullptr));
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          qb[nt][c * 4 + j][0] = o[2 * j];
-          qb[nt][c * 4 + j][1] = o[2 * j + 1];
+          qb[n][c * 4 + j][0] = o[2 * j];
+          qb[n][c * 4 + j][1] = o[2 * j + 1];
+        }
+        if (Q_SHARED) {
+          qs[(nt * NC * 2 + 2 * c) * 32 + lane] = make_uint4(o[0], o[1], o[2], o[3]);
+          qs[(nt * NC * 2 + 2 * c + 1) * 32 + lane] = make_uint4(o[4], o[5], o[6], o[7]);
         }
       }
+      if (Q_SHARED) {
+        if (tq == 0) q_back[nt * 8 + g] = back;
+      } else {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) qmul[n][i] = __shfl_sync(FULL_MASK, back, (2 * tq + i) * 4) * p.sl2;
+      }
+    }
+    if (Q_SHARED) __syncthreads();
+#pragma unroll
+    for (int nt = 0; nt < NG; ++nt) {
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        qmul[nt][i] = __shfl_sync(FULL_MASK, back, (2 * tq + i) * 4) * p.sl2;
+        if (Q_SHARED) qmul[nt][i] = q_back[nt * 8 + 2 * tq + i] * p.sl2;
         const int ri = row0 + nt * 8 + 2 * tq + i;
         lim[nt][i] = ri < rows ? len - seg.n_tok + ri / p.G + 1 : 0;
       }
@@ -455,13 +483,23 @@ __global__ void __launch_bounds__(NW * 32, ctas_per_sm(D, NG))
           const uint4 k0 = lds128(kp + page_off<D>(g, chunk)), k1 = lds128(kp + page_off<D>(g + 8, chunk));
           const uint32_t w0[4] = {k0.x, k0.y, k0.z, k0.w}, w1[4] = {k1.x, k1.y, k1.z, k1.w};
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            uint32_t a0, a1, a2, a3;
-            q8::decode4_h2<CODE>(w0[j], a0, a2);
-            q8::decode4_h2<CODE>(w1[j], a1, a3);
+          for (int j2 = 0; j2 < 2; ++j2) {
+            uint4 qv[NG];
+            if (Q_SHARED) {
 #pragma unroll
-            for (int nt = 0; nt < NG; ++nt)
-              Mma<__half>::run(acc[nt], a0, a1, a2, a3, qb[nt][c * 4 + j][0], qb[nt][c * 4 + j][1]);
+              for (int nt = 0; nt < NG; ++nt) qv[nt] = lds128(qs_lane + (nt * NC * 2 + 2 * c + j2) * 512);
+            }
+#pragma unroll
+            for (int j = 2 * j2; j < 2 * j2 + 2; ++j) {
+              uint32_t a0, a1, a2, a3;
+              q8::decode4_h2<CODE>(w0[j], a0, a2);
+              q8::decode4_h2<CODE>(w1[j], a1, a3);
+#pragma unroll
+              for (int nt = 0; nt < NG; ++nt)
+                Mma<__half>::run(acc[nt], a0, a1, a2, a3,
+                                 Q_SHARED ? (j & 1 ? qv[nt].z : qv[nt].x) : qb[Q_SHARED ? 0 : nt][c * 4 + j][0],
+                                 Q_SHARED ? (j & 1 ? qv[nt].w : qv[nt].y) : qb[Q_SHARED ? 0 : nt][c * 4 + j][1]);
+            }
           }
         }
         // V: tokens 2 tq, 2 tq + 1, 2 tq + 8, 2 tq + 9; this lane's D / 8 dims from D / 8 * g
@@ -687,7 +725,7 @@ constexpr int JT = 512;
 template <typename QT, int D, int NG, int RPC>
 __global__ void __launch_bounds__(JT) join_kernel(const Params p) {
   constexpr int ROWS = 8 * NG, LN = D / 4, ITEMS = RPC * LN, SUBS = ITEMS >= JT ? 1 : JT / ITEMS;
-  constexpr int CTAS = SMS * ctas_per_sm(D, NG), PER = (CTAS + 31) / 32;
+  constexpr int CTAS = SMS * ctas_per_sm(D, NG, false), PER = (CTAS + 31) / 32;
   __shared__ float weight[RPC][CTAS + 1];
   __shared__ float lsums[RPC], tops[RPC];
   __shared__ float4 sx[SUBS > 1 ? JT : 1];
@@ -780,11 +818,15 @@ int64_t group_bound(const ic_paged_attn_args& a, int rows) {
 // the 3 to 4 us of a second kernel, but a group is then split over no more than
 // 8 CTAs, or left whole when there are many groups: so only while the table's
 // width leaves a CTA at most MAX_CTA_PAGES pages.  (33 sessions x 19 tokens x 8
-// heads of 8 at 256 dims: shares of the line 859 us, a CTA per group 264.)
+// heads of 8 at 256 dims: shares of the line 859 us, a CTA per group 264 at the
+// time, 232 now.)
+// Powers of two: clusters of 3 and 6 do not fill the processor groups (96 groups
+// of 16 rows at 128 dims over 1400 keys: 21.1 us in 3s, 17.0 in 2s).
 constexpr int MAX_CTA_PAGES = 96;
 int cluster_size(const ic_paged_attn_args& a, int rows) {
-  const int64_t groups = group_bound(a, rows);
-  const int64_t cl = std::max<int64_t>(1, std::min<int64_t>(8, SMS * ctas_per_sm(a.head_dim, rows / 8) / groups));
+  const int64_t groups = group_bound(a, rows), slots = SMS * ctas_per_sm(a.head_dim, rows / 8, true);
+  int64_t cl = 1;
+  while (cl < 8 && 2 * cl * groups <= slots) cl *= 2;
   return a.table_width <= MAX_CTA_PAGES * cl && groups * cl <= 0x7fffffff ? static_cast<int>(cl) : 0;
 }
 
@@ -795,9 +837,9 @@ int launch(const Params& p, const ic_paged_attn_args& a, cudaStream_t st) {
   if ((rc = page_map(&mk, a.k, a.pool_tokens, p.H, D)) != IC_OK) return rc;
   if ((rc = page_map(&mv, a.v, a.pool_tokens, p.H, D)) != IC_OK) return rc;
   Params params = p;
-  const int smem = Layout<D, NG>::bytes(p.S);
   if (const int cl = p.few_rows == ALL_ROWS ? cluster_size(a, 8 * NG) : 0) {
     static PerDeviceLimit grouped_limit;
+    const int smem = Layout<D, NG, true>::bytes(p.S);
     auto kern = stream_kernel<QT, D, CODE, NG, true>;
     if ((rc = ensure_dynamic_smem(kern, smem, &grouped_limit)) != IC_OK) return rc;
     params.cluster = cl;
@@ -819,8 +861,9 @@ int launch(const Params& p, const ic_paged_attn_args& a, cudaStream_t st) {
   }
   auto kern = stream_kernel<QT, D, CODE, NG, false>;
   static PerDeviceLimit limit;
+  const int smem = Layout<D, NG, false>::bytes(p.S);
   if ((rc = ensure_dynamic_smem(kern, smem, &limit)) != IC_OK) return rc;
-  constexpr int ctas = SMS * ctas_per_sm(D, NG);
+  constexpr int ctas = SMS * ctas_per_sm(D, NG, false);
   void* args[] = {&mk, &mv, &params};
   if ((rc = launch_pdl(reinterpret_cast<const void*>(kern), dim3(ctas), dim3(NW * 32), smem, st, args,
                        "paged_attention (stream)")) != IC_OK)
@@ -853,14 +896,14 @@ int launch_dim(const Params& p, const ic_paged_attn_args& a, cudaStream_t st, bo
 }  // namespace
 
 int64_t stream_workspace(const ic_paged_attn_args& a) {
-  const int rows = stream_rows(static_cast<int64_t>(a.max_count) * (a.num_q_heads / a.num_kv_heads));
+  const int rows = stream_rows(static_cast<int64_t>(a.max_count) * (a.num_q_heads / a.num_kv_heads), a.head_dim);
   if (few_rows(a) == ALL_ROWS && cluster_size(a, rows) > 0) return 0;
-  const int64_t ctas = SMS * ctas_per_sm(a.head_dim, rows / 8);
+  const int64_t ctas = SMS * ctas_per_sm(a.head_dim, rows / 8, false);
   return 2 * ctas * rows * (a.head_dim + 2) * 4 + ctas * static_cast<int64_t>(sizeof(Task));
 }
 
 int launch_stream(const Params& p, const ic_paged_attn_args& a, cudaStream_t st) {
-  const bool one = stream_rows(static_cast<int64_t>(a.max_count) * p.G) == 8;
+  const bool one = stream_rows(static_cast<int64_t>(a.max_count) * p.G, a.head_dim) == 8;
   return a.q_dtype == IC_F16 ? launch_dim<__half>(p, a, st, one) : launch_dim<__nv_bfloat16>(p, a, st, one);
 }
 
