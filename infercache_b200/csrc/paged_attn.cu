@@ -79,7 +79,7 @@ int check(const ic_paged_attn_args* a) {
 // it does the work several times over.
 int few_rows(const ic_paged_attn_args& a) {
   const int64_t G = a.num_q_heads / a.num_kv_heads;
-  if (a.head_dim == 256 || a.max_count * G <= 64 || a.num_q_tokens * static_cast<int64_t>(a.num_q_heads) <= 4096)
+  if (a.max_count * G <= 64 || a.num_q_tokens * static_cast<int64_t>(a.num_q_heads) <= 4096)
     return ALL_ROWS;
   return 64;
 }

@@ -51,7 +51,10 @@ namespace {
 constexpr int TB = 128;                // query rows and keys per tile
 constexpr int SUB = TB * 64 * 2;       // one 64-column swizzled sub-tile: 16 KB
 constexpr int THREADS = 512;
-constexpr int RS = 5;                  // K / V ring slots
+// Query tiles per CTA, warps that convert codes, K / V ring slots.
+template <int D> constexpr int TILES = D == 256 ? 1 : 2;
+template <int D> constexpr int CONVERTERS = D == 256 ? 8 : 4;
+template <int D> constexpr int SLOTS = D == 256 ? 2 : 5;
 constexpr int NSC = 8;                 // key tiles whose scales are kept: the ring runs at most 3 ahead of the softmax
 constexpr int SORTED = 128;            // up to this many sessions are taken longest first
 constexpr float SLACK = 8.f, LIFT = 7.f;
@@ -59,7 +62,8 @@ constexpr float SLACK = 8.f, LIFT = 7.f;
 template <int D>
 struct Lay {
   static constexpr int TILE = D / 64 * SUB;
-  static constexpr int RING = 2 * TILE;
+  static constexpr int RS = SLOTS<D>;
+  static constexpr int RING = TILES<D> * TILE;
   static constexpr int SCALES = RING + RS * TILE;      // [NSC][3][8]: k scale, log2 v scale, 1 / v scale
   static constexpr int BARS = SCALES + NSC * 24 * 4;   // 16-byte aligned rows of 8
   static constexpr int NBAR = 22;
@@ -102,6 +106,8 @@ template <typename QT, int D, int CODE>
 __global__ void __launch_bounds__(THREADS, 1) tile_kernel(const Params p) {
   using L = Lay<D>;
   constexpr int NS = D / 64;  // 64-column sub-tiles of an operand row
+  constexpr int NT = TILES<D>, CW = CONVERTERS<D>, RS = L::RS;
+  constexpr int PW = 8 / CW;  // pages of a key tile that a converting warp takes
   extern __shared__ unsigned char smem_raw[];
   unsigned char* smem = smem_raw + ((1024 - (smem_addr(smem_raw) & 1023)) & 1023);
   const uint32_t sbase = smem_addr(smem);
@@ -125,9 +131,9 @@ __global__ void __launch_bounds__(THREADS, 1) tile_kernel(const Params p) {
   if (tid == 0) {
     *abort = 0;
     found[0] = -1;
-    mbar_init(q_full, 256);
+    mbar_init(q_full, NT * 128);
     for (int i = 0; i < RS; ++i) {
-      mbar_init(r_full + i, 128);
+      mbar_init(r_full + i, CW * 32);
       mbar_init(r_empty + i, 1);
     }
     for (int x = 0; x < 2; ++x) {
@@ -151,7 +157,7 @@ __global__ void __launch_bounds__(THREADS, 1) tile_kernel(const Params p) {
   const auto pairs_of = [&](int x) {
     int begin;
     const int rows = query_tokens(p, x, begin) * p.G;
-    return rows > p.few_rows ? (rows + 2 * TB - 1) / (2 * TB) : 0;
+    return rows > p.few_rows ? (rows + NT * TB - 1) / (NT * TB) : 0;
   };
   if (p.S <= SORTED) {
     int own = 0, held = 0;
@@ -210,8 +216,8 @@ __global__ void __launch_bounds__(THREADS, 1) tile_kernel(const Params p) {
   }
   int q_begin;
   const int n_tok = query_tokens(p, s, q_begin), rows = n_tok * p.G, len = held_tokens(p, s);
-  const int row_a = pair * 2 * TB;
-  const bool has_b = row_a + TB < rows;
+  const int row_a = pair * NT * TB;
+  const bool has_b = NT == 2 && row_a + TB < rows;
   // keys that row r sees: len - n_tok + r / G + 1; a tile's last row sets its range
   const auto tiles_of = [&](int row0) {
     const int last = min(row0 + TB, rows) - 1;
@@ -254,13 +260,17 @@ __global__ void __launch_bounds__(THREADS, 1) tile_kernel(const Params p) {
       // ---- O_a += P_a V(j), O_b += P_b V(j) -------------------------------------------
       bool ok = true;
       for (int j = 0; ok && j < n; ++j) {
+        // P first: it shows that S(j) is done, hence that the slot's last tenant was
+        // there; without that a parity alone cannot tell this phase from the one before
         const int u = u_v(j);
-        if (!(ok = one_wait(r_full + u % RS, (u / RS) & 1, p.status, abort))) break;
+        bool here = false;
         const uint32_t sv = sbase + L::RING + (u % RS) * L::TILE;
         for (int x = 0; x < 2; ++x) {
           if (j >= (x ? nb : na)) continue;
           for (int half = 0; half < 2; ++half) {
             if (!(ok = one_wait(p_full + 2 * x + half, j & 1, p.status, abort))) break;
+            if (!here && !(ok = one_wait(r_full + u % RS, (u / RS) & 1, p.status, abort))) break;
+            here = true;
             tc::fence_after();
 #pragma unroll
             for (int kk = 0; kk < TB / 32; ++kk)
@@ -275,10 +285,10 @@ __global__ void __launch_bounds__(THREADS, 1) tile_kernel(const Params p) {
       tc::commit(mma_done);
       mbar_wait_bounded(mma_done, 0, p.status);
     }
-  } else if (warp < 8) {
+  } else if (warp < 8 || (CW == 8 && warp >= 12)) {
     // ---- codes to operand tiles -----------------------------------------------------
     asm volatile("setmaxnreg.dec.sync.aligned.u32 96;");
-    const int cw = warp - 4, t8 = lane >> 2, c4 = lane & 3;
+    const int cw = warp < 8 ? warp - 4 : warp - 8, t8 = lane >> 2, c4 = lane & 3;
     const int32_t* trow = p.table + static_cast<int64_t>(s) * p.width;
     const int64_t plane = static_cast<int64_t>(h) * p.n_pages;
     const uint8_t* kc = static_cast<const uint8_t*>(p.k) + plane * q8::PAGE * D;
@@ -289,13 +299,13 @@ __global__ void __launch_bounds__(THREADS, 1) tile_kernel(const Params p) {
       j = is_v ? (u == total - 1 ? n - 1 : u / 2 - 1) : (u + 1) / 2;
       return is_v;
     };
-    // this warp's 32 tokens of a key tile are pages 2 cw and 2 cw + 1 of its eight
+    // this warp's tokens of a key tile are pages PW cw .. PW cw + PW - 1 of its eight
     const auto pages_at = [&](int u, int* id) {
       int j;
       what(u, j);
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int pg = j * 8 + cw * 2 + i;
+      for (int i = 0; i < PW; ++i) {
+        const int pg = j * 8 + cw * PW + i;
         id[i] = -1;
         if (u < total && pg * q8::PAGE < len) {
           const int x = trow[pg];
@@ -310,8 +320,8 @@ __global__ void __launch_bounds__(THREADS, 1) tile_kernel(const Params p) {
     // them); as soon as a vector is stored, the one two positions on is loaded in
     // its place, so a load has two tiles' time to arrive.
     struct Held {
-      uint4 reg[4][NS];
-      float ks, vs;   // lanes 0, 1: the scales of pages 2 cw, 2 cw + 1 ...
+      uint4 reg[2 * PW][NS];
+      float ks, vs;   // lane i < PW: the scales of this warp's page i ...
       bool mine;      // ... and whether there is such a page
     };
     const uint32_t lane_codes = t8 * D + c4 * 16;
@@ -324,7 +334,7 @@ __global__ void __launch_bounds__(THREADS, 1) tile_kernel(const Params p) {
     const auto page_at = [&](int u, const int* id, int i) -> At {
       int j;
       const uint8_t* codes = what(u, j) ? vc : kc;
-      const int left = len - (j * 8 + cw * 2 + i) * q8::PAGE;
+      const int left = len - (j * 8 + cw * PW + i) * q8::PAGE;
       return At{codes + static_cast<int64_t>(max(id[i], 0)) * (q8::PAGE * D) + lane_codes, id[i] < 0 ? 0 : min(left, q8::PAGE)};
     };
     const auto load_one = [&](const At& at, int g, int sub) -> uint4 {
@@ -332,33 +342,33 @@ __global__ void __launch_bounds__(THREADS, 1) tile_kernel(const Params p) {
       return *reinterpret_cast<const uint4*>(at.ptr + (g & 1) * 8 * D + sub * 64);
     };
     const auto load_scales = [&](const int* id, Held& b) {
-      const int page = id[lane & 1];
-      b.mine = lane < 2 && page >= 0;
+      const int page = id[PW == 1 ? 0 : lane & 1];
+      b.mine = lane < PW && page >= 0;
       b.ks = b.vs = 1.f;
       if (b.mine) {
         b.ks = p.k_scale[plane + page];
         b.vs = p.v_scale[plane + page];
       }
     };
-    int next[2], later[2];  // page ids two and three positions on
+    int next[PW], later[PW];  // page ids two and three positions on
     const auto step = [&](int u, Held& b) -> bool {
       pages_at(u + 3, later);
       const int st = u % RS;
       if (u >= RS && !warp_wait(r_empty + st, ((u / RS) - 1) & 1, p.status, abort)) return false;
       int j;
       const bool is_v = what(u, j);
-      if (!is_v && lane < 2) {
-        float* sc = scales + (j % NSC) * 24 + cw * 2 + lane;
+      if (!is_v && lane < PW) {
+        float* sc = scales + (j % NSC) * 24 + cw * PW + lane;
         const float k1 = fmaxf(b.ks, 7.8886090522101181e-31f), v1 = fmaxf(b.vs, 7.8886090522101181e-31f);
         sc[0] = k1;                                   // at least 2^-100: a zero scale stays harmless
         sc[8] = b.mine ? log2f(v1) : -INFINITY;       // no page: no weight
         sc[16] = b.mine ? 1.f / v1 : 0.f;
       }
       load_scales(next, b);
-      const At at[2] = {page_at(u + 2, next, 0), page_at(u + 2, next, 1)};
-      const uint32_t dst = sbase + L::RING + st * L::TILE + (cw * 32 + t8) * 128 + (((2 * c4) ^ t8) << 4);
+      const At at[2] = {page_at(u + 2, next, 0), page_at(u + 2, next, PW - 1)};
+      const uint32_t dst = sbase + L::RING + st * L::TILE + (cw * PW * 16 + t8) * 128 + (((2 * c4) ^ t8) << 4);
 #pragma unroll
-      for (int g = 0; g < 4; ++g) {
+      for (int g = 0; g < 2 * PW; ++g) {
 #pragma unroll
         for (int sub = 0; sub < NS; ++sub) {
           const uint4 w = b.reg[g][sub];
@@ -374,17 +384,17 @@ __global__ void __launch_bounds__(THREADS, 1) tile_kernel(const Params p) {
       }
       fence_proxy_async_smem();
       tc::mbar_arrive(r_full + st);
-      next[0] = later[0];
-      next[1] = later[1];
+#pragma unroll
+      for (int i = 0; i < PW; ++i) next[i] = later[i];
       return true;
     };
     Held even, odd;
     const auto fill = [&](int u, Held& b) {
       pages_at(u, next);
       load_scales(next, b);
-      const At at[2] = {page_at(u, next, 0), page_at(u, next, 1)};
+      const At at[2] = {page_at(u, next, 0), page_at(u, next, PW - 1)};
 #pragma unroll
-      for (int g = 0; g < 4; ++g)
+      for (int g = 0; g < 2 * PW; ++g)
 #pragma unroll
         for (int sub = 0; sub < NS; ++sub) b.reg[g][sub] = load_one(at[g >> 1], g, sub);
     };
@@ -408,37 +418,54 @@ __global__ void __launch_bounds__(THREADS, 1) tile_kernel(const Params p) {
     float qmul = fabsf(p.sl2);
     if (nx > 0) {
       const QT* src = static_cast<const QT*>(p.q) + tok * p.q_stride_t + head * p.q_stride_h;
-      uint4 w[D / 8];
+      // at most 16 vectors at a time; two passes where the row has more (256 dims)
+      constexpr int QC = D / 8 < 16 ? D / 8 : 16;
+      uint4 w[QC];
+      const auto load_q = [&](int c0) {
 #pragma unroll
-      for (int c = 0; c < D / 8; ++c) w[c] = valid ? reinterpret_cast<const uint4*>(src)[c] : make_uint4(0, 0, 0, 0);
-      if (std::is_same<QT, __nv_bfloat16>::value) {
+        for (int c = 0; c < QC; ++c) w[c] = valid ? reinterpret_cast<const uint4*>(src)[c0 + c] : make_uint4(0, 0, 0, 0);
+      };
+      constexpr bool SCALE_Q = std::is_same<QT, __nv_bfloat16>::value;
+      float f = 1.f;
+      if (SCALE_Q) {
         // bf16 to fp16: a power of two brings the row's largest finite value into [2^13, 2^14)
         uint32_t m = 0;
+        for (int c0 = D / 8 - QC; c0 >= 0; c0 -= QC) {
+          load_q(c0);
 #pragma unroll
-        for (int c = 0; c < D / 8; ++c) {
-          const uint32_t* u = reinterpret_cast<const uint32_t*>(&w[c]);
+          for (int c = 0; c < QC; ++c) {
+            const uint32_t* u = reinterpret_cast<const uint32_t*>(&w[c]);
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const uint32_t lo = (u[i] << 16) & 0x7fffffffu, hi = u[i] & 0x7fff0000u;
-            m = max(m, lo < 0x7f800000u ? lo : 0u);
-            m = max(m, hi < 0x7f800000u ? hi : 0u);
+            for (int i = 0; i < 4; ++i) {
+              const uint32_t lo = (u[i] << 16) & 0x7fffffffu, hi = u[i] & 0x7fff0000u;
+              m = max(m, lo < 0x7f800000u ? lo : 0u);
+              m = max(m, hi < 0x7f800000u ? hi : 0u);
+            }
           }
         }
         const int e = max(static_cast<int>(m >> 23) - 126, -100);
-        const float f = q8::two_to(14 - e);
+        f = q8::two_to(14 - e);
         qmul *= q8::two_to(e - 14);
-#pragma unroll
-        for (int c = 0; c < D / 8; ++c) {
-          uint32_t* u = reinterpret_cast<uint32_t*>(&w[c]);
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-            u[i] = half2_bits(__uint_as_float(u[i] << 16) * f, __uint_as_float(u[i] & 0xffff0000u) * f);
-        }
+      } else {
+        load_q(0);
       }
 #pragma unroll
-      for (int c = 0; c < D / 8; ++c)
-        sts128(sbase + x * L::TILE + (c >> 3) * SUB + r * 128 + (((c & 7) ^ (r & 7)) << 4), w[c].x ^ flip, w[c].y ^ flip,
-               w[c].z ^ flip, w[c].w ^ flip);
+      for (int c0 = 0; c0 < D / 8; c0 += QC) {
+        if (c0 > 0) load_q(c0);
+        if (SCALE_Q) {
+#pragma unroll
+          for (int c = 0; c < QC; ++c) {
+            uint32_t* u = reinterpret_cast<uint32_t*>(&w[c]);
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              u[i] = half2_bits(__uint_as_float(u[i] << 16) * f, __uint_as_float(u[i] & 0xffff0000u) * f);
+          }
+        }
+#pragma unroll
+        for (int c = 0; c < QC; ++c)
+          sts128(sbase + x * L::TILE + ((c0 + c) >> 3) * SUB + r * 128 + (((c & 7) ^ (r & 7)) << 4), w[c].x ^ flip,
+                 w[c].y ^ flip, w[c].z ^ flip, w[c].w ^ flip);
+      }
     }
     fence_proxy_async_smem();
     tc::mbar_arrive(q_full);
@@ -572,7 +599,7 @@ int launch(const Params& p, const ic_paged_attn_args& a, cudaStream_t st) {
   int rc;
   if ((rc = ensure_dynamic_smem(kern, Lay<D>::BYTES, &limit)) != IC_OK) return rc;
   // at most this many (session, pair) units, whatever the sessions' counts
-  const int64_t units = static_cast<int64_t>(a.num_q_tokens) * p.G / (2 * TB) + std::min<int64_t>(p.S, a.num_q_tokens);
+  const int64_t units = static_cast<int64_t>(a.num_q_tokens) * p.G / (TILES<D> * TB) + std::min<int64_t>(p.S, a.num_q_tokens);
   Params params = p;
   void* args[] = {&params};
   return launch_pdl(reinterpret_cast<const void*>(kern), dim3(static_cast<unsigned>(units * p.H)), dim3(THREADS),
@@ -583,7 +610,9 @@ template <typename QT>
 int launch_q(const Params& p, const ic_paged_attn_args& a, cudaStream_t st) {
   if (a.head_dim == 64)
     return a.code_dtype == IC_E4M3 ? launch<QT, 64, IC_E4M3>(p, a, st) : launch<QT, 64, IC_I8>(p, a, st);
-  return a.code_dtype == IC_E4M3 ? launch<QT, 128, IC_E4M3>(p, a, st) : launch<QT, 128, IC_I8>(p, a, st);
+  if (a.head_dim == 128)
+    return a.code_dtype == IC_E4M3 ? launch<QT, 128, IC_E4M3>(p, a, st) : launch<QT, 128, IC_I8>(p, a, st);
+  return a.code_dtype == IC_E4M3 ? launch<QT, 256, IC_E4M3>(p, a, st) : launch<QT, 256, IC_I8>(p, a, st);
 }
 
 }  // namespace

@@ -425,6 +425,33 @@ def test_attention_prompts_hard_cases(codes):
     assert torch.equal(got, want)
 
 
+@pytest.mark.parametrize("codes", CODES)
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("H,G", [(1, 8), (2, 5), (3, 1), (1, 16)])
+def test_attention_prompts_of_256_dims(codes, dtype, H, G):
+    """One query tile per CTA, a ring of two key tiles."""
+    x = attention_inputs(H * G, [n * 3 for n in TILE_LENS], [c * 3 for c in TILE_COUNTS], H, G, 256, codes, dtype)
+    assert x[0].shape[0] * x[0].shape[1] > 4096 or H * G < 4
+    assert check_attention(x)[2] == 0
+
+
+def test_attention_prompts_of_256_dims_hard_cases():
+    x = attention_inputs(3, TILE_LENS, TILE_COUNTS, 2, 4, 256, CODES[0], torch.bfloat16, k_spread=6, v_spread=20)
+    assert x[0].shape[0] * x[0].shape[1] > 4096
+    out, _, _ = check_attention(x)
+    check_attention((x[0] * 1e30,) + x[1:], scale=-1e-30)
+    q = x[0].clone()
+    q[17, 3, 200] = math.nan
+    from infercache_b200.paged_ops import paged_attention
+    got = paged_attention(q, *x[1:])
+    assert bool(torch.isnan(got[17, 3]).all())
+    got[17, 3] = out[17, 3]
+    assert torch.equal(got, out)
+    t = x[5].clone()
+    t[0, 2], t[5, 9] = -1, 10 ** 9
+    assert check_attention(x[:5] + (t,) + x[6:])[2] == BAD_ROW
+
+
 def test_attention_many_sessions_of_prompts():
     """More sessions than one pass of a CTA's threads looks through."""
     rng = np.random.default_rng(1)
