@@ -73,13 +73,18 @@ int check(const ic_paged_attn_args* a) {
 }  // namespace
 
 // Sessions with at most this many query rows per KV head are the streaming
-// kernel's.  It reads a session's pages once per 16 rows, the tile kernel
-// converts them once per 256 but gives each (session, KV head, 256 rows) to one
-// CTA: below some 20 such CTAs the streaming kernel's even shares win although
-// it does the work several times over.
+// kernel's.  It reads a session's pages once per 8 or 16 rows, the tile kernel
+// converts them once per 256 (128 at 256 dims) but gives each (session, KV head,
+// that many rows) to one CTA: below some 16 such CTAs the streaming kernel's even
+// shares win although it does the work several times over.  Measured, streaming /
+// tiles: one session of 8192 tokens, 2 heads of 8, 256 new tokens (4096 rows in
+// all) 119 / 133 us at 128 dims, 196 / 139 at 256; 384 new ones 172 / 134 at 128;
+// 128 new ones (2048 rows) 104 / 138 at 256; 16 sessions of 500 with 24 new, 4
+// heads of 4 (6144 rows) 26 / 18 at 128.
 int few_rows(const ic_paged_attn_args& a) {
   const int64_t G = a.num_q_heads / a.num_kv_heads;
-  if (a.max_count * G <= 64 || a.num_q_tokens * static_cast<int64_t>(a.num_q_heads) <= 4096)
+  if (a.max_count * G <= 64 ||
+      a.num_q_tokens * static_cast<int64_t>(a.num_q_heads) <= (a.head_dim == 256 ? 2048 : 4096))
     return ALL_ROWS;
   return 64;
 }
