@@ -140,16 +140,17 @@ __device__ __forceinline__ void store_codes(uint32_t* dst, const uint32_t* o) {
 }
 
 // A page's source rows pass through CHUNK vectors per lane twice, for the
-// maximum and for the codes; the second reading hits the cache and a run of one
-// or two tokens needs none.  Holding the whole page instead (8 to 32 vectors)
-// is 3 % faster for long prompts (write-out of 16 x 2k tokens: 599 against
-// 617 us) but leaves a third of the warps: 78 against 65 us for one token of
-// 149 sessions in 28 layers, 29 against 12 us for 24 tokens of each in one.
-constexpr int CHUNK = 4;
+// maximum and for the codes; the second reading hits the cache and a run that
+// fits needs none.  4 leave more loads of short runs in flight: one token of 149
+// sessions in 28 layers 65 us (8: 78), 4 to 10 of 108 in 36 44 (51); 8 take a
+// 16-bit page of 128 dims whole: 16 prompts of 2k tokens in 36 layers, written and
+// read back, 596 us (4: 616), 4 of 1024 x 4 heads 150 (161).  Both with 64
+// registers a thread (80: 652 us for the prompts).
+constexpr int64_t BIG_WRITE = 1 << 18;  // tokens x layers x heads from which it is 8
 
 // `cnt` tokens, source rows src + t * stride (elements), into slots off ..
 // off + cnt - 1 of the page at `page` (16 rows of D codes).
-template <typename T, int D, int CODE>
+template <typename T, int D, int CODE, int CHUNK>
 __device__ __forceinline__ void write_run(const T* src, int64_t stride, int cnt, int off, uint8_t* page, float* scale_p,
                                           int32_t* status, int lane) {
   constexpr int E = VE<T>, W = E / 4;         // elements and code words per vector
@@ -252,8 +253,8 @@ __device__ __forceinline__ void write_run(const T* src, int64_t stride, int cnt,
   if (lane == 0) *scale_p = q8::two_to(e);
 }
 
-template <typename T, int D, int CODE>
-__global__ void __launch_bounds__(WARPS * 32) write_kernel(const __grid_constant__ Batch b) {
+template <typename T, int D, int CODE, int CHUNK>
+__global__ void __launch_bounds__(WARPS * 32, 8) write_kernel(const __grid_constant__ Batch b) {
   grid_dependency_wait();
   grid_launch_dependents();
   const int lane = threadIdx.x & 31;
@@ -275,7 +276,7 @@ __global__ void __launch_bounds__(WARPS * 32) write_kernel(const __grid_constant
     const int64_t t0 = max(page0 - r.start, int64_t{0}), t1 = min(page0 + q8::PAGE - r.start, r.n);
     const int64_t slot = slot_of(r, t0);
     if (slot < 0 || slot >= b.pool_tokens) return;
-    write_run<T, D, CODE>(buf + t0 * r.stride_t, r.stride_t, static_cast<int>(t1 - t0),
+    write_run<T, D, CODE, CHUNK>(buf + t0 * r.stride_t, r.stride_t, static_cast<int>(t1 - t0),
                           static_cast<int>(slot % q8::PAGE), codes + slot / q8::PAGE * (q8::PAGE * D),
                           scales + slot / q8::PAGE, b.status, lane);
     return;
@@ -296,7 +297,7 @@ __global__ void __launch_bounds__(WARPS * 32) write_kernel(const __grid_constant
     const int32_t s0 = __shfl_sync(FULL_MASK, slot, j);
     const uint32_t rest = ~(cont >> j >> 1);  // bit k: token j + 1 + k does not go on
     const int cnt = min(__ffs(rest), q8::PAGE - s0 % q8::PAGE);
-    write_run<T, D, CODE>(buf + (w0 - 1 + j) * r.stride_t, r.stride_t, cnt, s0 % q8::PAGE,
+    write_run<T, D, CODE, CHUNK>(buf + (w0 - 1 + j) * r.stride_t, r.stride_t, cnt, s0 % q8::PAGE,
                           codes + static_cast<int64_t>(s0 / q8::PAGE) * (q8::PAGE * D), scales + s0 / q8::PAGE, b.status,
                           lane);
     __syncwarp();
@@ -439,14 +440,18 @@ void fill_batch(const ic_page_q8_args* a, Batch& b) {
   }
 }
 
-template <typename T, int D>
+template <typename T, int D, int CHUNK>
 const void* write_fn(int code) {
-  return code == IC_E4M3 ? reinterpret_cast<const void*>(write_kernel<T, D, IC_E4M3>)
-                         : reinterpret_cast<const void*>(write_kernel<T, D, IC_I8>);
+  return code == IC_E4M3 ? reinterpret_cast<const void*>(write_kernel<T, D, IC_E4M3, CHUNK>)
+                         : reinterpret_cast<const void*>(write_kernel<T, D, IC_I8, CHUNK>);
+}
+template <typename T, int CHUNK>
+const void* write_fn_c(int d, int code) {
+  return d == 64 ? write_fn<T, 64, CHUNK>(code) : d == 128 ? write_fn<T, 128, CHUNK>(code) : write_fn<T, 256, CHUNK>(code);
 }
 template <typename T>
-const void* write_fn_d(int d, int code) {
-  return d == 64 ? write_fn<T, 64>(code) : d == 128 ? write_fn<T, 128>(code) : write_fn<T, 256>(code);
+const void* write_fn_d(int d, int code, bool big) {
+  return big ? write_fn_c<T, 8>(d, code) : write_fn_c<T, 4>(d, code);
 }
 template <typename T, int D>
 const void* read_fn(int code) {
@@ -490,9 +495,10 @@ extern "C" int ic_page_write_q8(const ic_page_q8_args* a, void* stream) {
     set_last_error("page_write_q8: too many tokens for one launch");
     return IC_ERR_UNSUPPORTED;
   }
-  const void* fn = a->buf_dtype == IC_F32   ? write_fn_d<float>(D, a->pool.dtype)
-                   : a->buf_dtype == IC_F16 ? write_fn_d<__half>(D, a->pool.dtype)
-                                            : write_fn_d<__nv_bfloat16>(D, a->pool.dtype);
+  const bool big = tokens * planes > BIG_WRITE;
+  const void* fn = a->buf_dtype == IC_F32   ? write_fn_d<float>(D, a->pool.dtype, big)
+                   : a->buf_dtype == IC_F16 ? write_fn_d<__half>(D, a->pool.dtype, big)
+                                            : write_fn_d<__nv_bfloat16>(D, a->pool.dtype, big);
   void* p[] = {&b};
   return launch_pdl(fn, dim3(static_cast<unsigned>(blocks), planes, 2), dim3(WARPS * 32), 0,
                     static_cast<cudaStream_t>(stream), p, "page_write_q8");
