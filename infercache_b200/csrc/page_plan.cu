@@ -53,7 +53,7 @@ __device__ __forceinline__ int32_t pages_of(int64_t tokens) {
   return static_cast<int32_t>((tokens + q8::PAGE - 1) / q8::PAGE);
 }
 
-// A warp's tokens [i0, i1), i0 a multiple of WT.  len[s] is session s's length
+// A warp's tokens [i0, i1), i0 a multiple of 32.  len[s] is session s's length
 // before the call (-1 when it was denied), rank[s] its first new page's rank,
 // `top` the stack's height before the call.
 __device__ __forceinline__ void plan_tokens(const ic_page_plan_args& a, const int32_t* q_start, const int32_t* len,
@@ -114,9 +114,15 @@ __device__ __forceinline__ void plan_tokens(const ic_page_plan_args& a, const in
     for (int j = 0; j < TPT; ++j) {
       const int64_t i = i0 + 32 * j + lane;
       if (i >= i1) break;
-      while (i >= xe && x + 1 < S) {
-        ++x;
-        xb = xe;
+      if (i >= xe && x + 1 < S) {  // the next session, mostly; else the last that begins at or before i
+        int a0 = x + 1, a1 = S;
+        if (q_start[a0 + 1] > i) a1 = a0 + 1;
+        while (a1 - a0 > 1) {
+          const int mid = (a0 + a1) >> 1;
+          if (q_start[mid] <= i) a0 = mid; else a1 = mid;
+        }
+        x = a0;
+        xb = q_start[x];
         xe = q_start[x + 1];
       }
       int32_t slot = -1, pos = -1;  // positions fit: a table row holds fewer than 2^31 tokens
@@ -136,8 +142,8 @@ __device__ __forceinline__ void plan_tokens(const ic_page_plan_args& a, const in
 }
 
 // `fused`: the sessions fit one pass of the threads and the tokens are
-// finished here, from shared memory.
-__global__ void __launch_bounds__(PT) plan_rows_kernel(const ic_page_plan_args a, int fused) {
+// finished here, from shared memory, `per_warp` consecutive ones by each warp.
+__global__ void __launch_bounds__(PT) plan_rows_kernel(const ic_page_plan_args a, int fused, int per_warp) {
   __shared__ int64_t warp_sums[32];
   __shared__ int32_t taken_s;
   __shared__ int32_t qs[PT + 1], len_s[PT], rank_s[PT];
@@ -192,12 +198,12 @@ __global__ void __launch_bounds__(PT) plan_rows_kernel(const ic_page_plan_args a
   if (__syncthreads_or(bad) && threadIdx.x == 0 && a.dev_status) atomicOr(a.dev_status, IC_DEVFLAG_NO_PAGES);
   if (threadIdx.x == 0) *a.free_count_out = top - taken_s;
   if (fused) {
-    const int64_t i0 = static_cast<int64_t>(threadIdx.x >> 5) * WT;
-    plan_tokens(a, qs, len_s, rank_s, 1, top, i0, min(i0 + WT, static_cast<int64_t>(a.total)));
+    const int64_t i0 = static_cast<int64_t>(threadIdx.x >> 5) * per_warp;
+    plan_tokens(a, qs, len_s, rank_s, 1, top, i0, min(i0 + per_warp, static_cast<int64_t>(a.total)));
   }
 }
 
-// Each warp takes `per_warp` consecutive tokens (a multiple of WT).
+// Each warp takes `per_warp` consecutive tokens (a multiple of 32).
 __global__ void __launch_bounds__(256) plan_tokens_kernel(const ic_page_plan_args a, int64_t per_warp) {
   extern __shared__ int32_t qs[];
   grid_dependency_wait();
@@ -281,13 +287,21 @@ extern "C" int ic_page_plan(const ic_page_plan_args* a, void* stream) {
   // and scans over idle warps would be most of a decode tick's plan
   int threads = a->num_sessions < ic::PT ? (a->num_sessions + 31) / 32 * 32 : ic::PT;
   if (fused) threads = max(threads, (a->total + ic::WT - 1) / ic::WT * 32);
-  void* p1[] = {&args, &fused};
+  // A warp walks its tokens 32 at a time and waits for each step's loads: spread
+  // them over the warps there are (a token each of 1000 sessions: 7.2 us; 256
+  // tokens to a warp: 14.5), but keep the 256 that are taken at once where
+  // sessions bring long runs.
+  const auto spread = [](int64_t each) {
+    return each <= ic::WT / 2 ? (each + 31) / 32 * 32 : (each + ic::WT - 1) / ic::WT * ic::WT;
+  };
+  int fused_per_warp = static_cast<int>(spread((a->total + threads / 32 - 1) / (threads / 32)));
+  void* p1[] = {&args, &fused, &fused_per_warp};
   int rc = ic::launch_pdl(reinterpret_cast<const void*>(ic::plan_rows_kernel), dim3(1), dim3(threads), 0, st, p1,
                           "page_plan (sessions)");
   if (rc != IC_OK || fused) return rc;
   // one wave of 8 CTAs per SM at most: a CTA copies q_start before it begins
   const int64_t warps = static_cast<int64_t>(148) * 8 * 8;
-  int64_t per_warp = ((a->total + warps - 1) / warps + ic::WT - 1) / ic::WT * ic::WT;
+  int64_t per_warp = spread((a->total + warps - 1) / warps);
   const int64_t per_cta = 8 * per_warp;
   void* p2[] = {&args, &per_warp};
   return ic::launch_pdl(reinterpret_cast<const void*>(ic::plan_tokens_kernel),
