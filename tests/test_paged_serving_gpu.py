@@ -63,6 +63,19 @@ def test_plan(S, width, max_len, max_count, free):
     check_plan(lens, counts, table, fr, sum(counts), commit=True)
 
 
+@pytest.mark.parametrize("S,total_free", [(1000, 700), (1025, 5000), (3000, 2000), (8192, 9000)])
+@pytest.mark.parametrize("top", [1, 3])
+def test_plan_many_sessions_of_few_tokens(S, total_free, top):
+    """Most sessions bring nothing or one token: a warp's tokens are many
+    sessions', with runs of empty ones between them."""
+    lens, counts, table, fr = plan_inputs(S + top, S, 4, 40, top, total_free)
+    counts = [c if i % 7 else 0 for i, c in enumerate(counts)]
+    counts[3:200] = [0] * 197
+    counts[300] = 24 if lens[300] <= 40 else 0
+    check_plan(lens, counts, table, fr, sum(counts))
+    check_plan(lens, counts, table, fr, sum(counts) + 5)
+
+
 def test_plan_edges():
     # exactly full table rows and pages, nothing to add, an empty total
     check_plan([16, 0, 31], [16, 32, 1], [[3, -1], [-1, -1], [1, 0]], [9, 8, 7], 49)
