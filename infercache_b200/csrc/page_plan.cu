@@ -10,6 +10,9 @@
 // read, so a large admission is bound by HBM writes and spreads over the GPU
 // in a second kernel, while a decode tick's few tokens are finished by the
 // scanning CTA itself (a second launch would cost more than the work).
+// Measured (B200): 16 sessions of one token 7.1 us (host time), 1000 as much; 512
+// prompts of 256 to 32768 tokens, 8.5 million in all, 25 us, 4.2 TB/s of stores
+// and some 4 us for the two kernels to begin.
 #include "common.cuh"
 #include "launch.cuh"
 #include "q8.cuh"
