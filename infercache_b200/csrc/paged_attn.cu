@@ -75,18 +75,20 @@ int check(const ic_paged_attn_args* a) {
 // Sessions with at most this many query rows per KV head are the streaming
 // kernel's.  It reads a session's pages once per 8 or 16 rows, the tile kernel
 // converts them once per 256 (128 at 256 dims) but gives each (session, KV head,
-// that many rows) to one CTA: below some 16 such CTAs the streaming kernel's even
-// shares win although it does the work several times over.  Measured, streaming /
-// tiles: one session of 8192 tokens, 2 heads of 8, 256 new tokens (4096 rows in
-// all) 119 / 133 us at 128 dims, 196 / 139 at 256; 384 new ones 172 / 134 at 128;
-// 128 new ones (2048 rows) 104 / 138 at 256; 16 sessions of 500 with 24 new, 4
-// heads of 4 (6144 rows) 26 / 18 at 128.
+// that many rows) to one CTA.  Two conditions follow: the call's rows have to
+// amount to enough CTAs (below some 16 the streaming kernel's even shares win
+// although it does the work several times over), and the session's to three or
+// more of its row tiles.  Measured, streaming / tiles, in us:
+//   rows in all, one session of 8192 tokens, 2 heads of 8:
+//     128 dims: 4096 119 / 133, 6144 172 / 134; 256 dims: 2048 104 / 138, 4096 196 / 139
+//   rows per session, 64 sessions of 4000 tokens, 2 to 4 heads:
+//     128 dims: 36 102 / 96, 48 103 / 95, 64 132 / 94 (40 sessions of 3000 tokens,
+//     35 rows, a second wave of tiles: 100 / 127); 256 dims: 16 117 / 164, 24 213 /
+//     165, 36 164 / 90, 64 214 / 91
 int few_rows(const ic_paged_attn_args& a) {
-  const int64_t G = a.num_q_heads / a.num_kv_heads;
-  if (a.max_count * G <= 64 ||
-      a.num_q_tokens * static_cast<int64_t>(a.num_q_heads) <= (a.head_dim == 256 ? 2048 : 4096))
-    return ALL_ROWS;
-  return 64;
+  const int64_t G = a.num_q_heads / a.num_kv_heads, rows = a.num_q_tokens * static_cast<int64_t>(a.num_q_heads);
+  const int few = a.head_dim == 256 ? 16 : 40;
+  return a.max_count * G <= few || rows <= (a.head_dim == 256 ? 2048 : 4096) ? ALL_ROWS : few;
 }
 
 int page_map(CUtensorMap* m, const void* codes, int64_t pool_tokens, int heads, int D) {

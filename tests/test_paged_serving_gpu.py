@@ -357,6 +357,26 @@ def test_attention_wide_tables_share_the_line(seed, S, G, D):
     assert status == 0
 
 
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("G", [2, 9])
+@pytest.mark.parametrize("width", [0, 1200])
+def test_attention_of_4096_sessions(D, G, width):
+    """The most sessions a call takes, most of them without a token this tick."""
+    lens = [(7 * i) % 45 for i in range(4096)]
+    counts = [1 if i % 31 == 5 and n else 0 for i, n in enumerate(lens)]
+    q, k, v, ks, vs, table, n, start = attention_inputs(D + G, lens, counts, 1, G, D, CODES[G % 2], torch.float16)
+    if width:
+        wide = torch.full((4096, width), -1, dtype=torch.int32, device="cuda")
+        wide[:, :table.shape[1]] = table
+        table = wide
+    assert check_attention((q, k, v, ks, vs, table, n, start), max_count=1)[2] == 0
+    from infercache_b200._lib import Unsupported
+    from infercache_b200.paged_ops import paged_attention
+    more = [torch.cat([x, x[:1]]) for x in (table, n)]
+    with pytest.raises(Unsupported):
+        paged_attention(q, k, v, ks, vs, *more, torch.cat([start, start[-1:]]))
+
+
 def test_two_calls_at_once_keep_apart():
     """Calls on two streams, whose workspaces and outputs are their own."""
     from infercache_b200.paged_ops import paged_attention
