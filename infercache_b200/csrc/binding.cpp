@@ -56,6 +56,11 @@ int64_t integer(PyObject* o) {
   if (v == -1 && PyErr_Occurred()) throw Raised();
   return v;
 }
+bool truth(PyObject* o) {
+  const int v = PyObject_IsTrue(o);
+  if (v < 0) throw Raised();
+  return v != 0;
+}
 double number(PyObject* o) {
   const double v = PyFloat_AsDouble(o);
   if (v == -1.0 && PyErr_Occurred()) throw Raised();
@@ -233,7 +238,7 @@ PyObject* py_page_plan(PyObject*, PyObject* const* a, Py_ssize_t n) {
       bad(name, "lens must be [S], block_table [S, width] and free_pages [P]");
     const int64_t S = lens.size(0), W = table.size(1), P = pages.size(0), total = integer(a[5]);
     if (total < 0 || total > 0x7fffffff) bad(name, "total must be in [0, 2^31), got " + std::to_string(total));
-    const bool commit = PyObject_IsTrue(a[6]) == 1;
+    const bool commit = truth(a[6]);
     ic_page_plan_args x = {};
     int32_t* lens_p = state(name, "lens", lens, dev, {S});
     int32_t* count_p = state(name, "free_count", count, dev, {1});
@@ -413,7 +418,7 @@ PyObject* py_paged_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
           !aligned16(out))
         bad(name, "out must be a contiguous, 16-byte aligned tensor like q");
     }
-    const bool want_lse = PyObject_IsTrue(a[11]) == 1;
+    const bool want_lse = truth(a[11]);
     if (want_lse) lse = fresh({N, Hq}, at::kFloat, c.dev);
     if (N > 0 && S > 0) {
       if (!rows16(q)) q = q.clone(at::MemoryFormat::Contiguous);

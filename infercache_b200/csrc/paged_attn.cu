@@ -150,7 +150,6 @@ extern "C" int ic_paged_attention(const ic_paged_attn_args* a, void* stream) {
   p.n_pages = static_cast<int32_t>(a->pool_tokens / q8::PAGE);
   p.n_q = a->num_q_tokens;
   p.few_rows = paged::few_rows(*a);
-  p.min_share = 32;
   p.sl2 = a->scale * paged::LOG2E;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (p.few_rows != paged::ALL_ROWS && (rc = paged::launch_tile(p, *a, st)) != IC_OK) return rc;

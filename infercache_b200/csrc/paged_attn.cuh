@@ -31,7 +31,6 @@ struct Params {
   int32_t S, width, Hq, H, G, n_pages;
   int32_t n_q;                // rows of q: sessions are clipped to them
   int32_t few_rows;           // sessions with at most this many rows are the streaming kernel's, the others the tile kernel's
-  int32_t min_share;          // streaming kernel: fewest pages per CTA
   int32_t cluster;            // streaming kernel: CTAs per group where each has a cluster
   float sl2;                  // scale * log2(e)
 };

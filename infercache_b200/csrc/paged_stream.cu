@@ -62,6 +62,9 @@ constexpr int NW = 8;                 // warps per CTA
 // groups of one page: 83 sessions of 6 tokens, 4 heads of 16: 98 us, now 25; the 64
 // sessions of up to 8k tokens: 62 us, now 58.)
 constexpr int OVERHEAD = 24;
+// The fewest units a CTA takes; more than OVERHEAD, so that a share holds a page.
+constexpr int MIN_SHARE = 32;
+static_assert(MIN_SHARE > OVERHEAD, "a share that begins before a group's first page reaches it");
 constexpr float TINY = 7.8886090522101181e-31f;  // 2^-100
 constexpr float SLACK = 8.f;          // u may pass M by this much
 constexpr float LIFT = 7.f;           // P' = 2^(u - M + LIFT): at most 2^15
@@ -256,7 +259,7 @@ __global__ void __launch_bounds__(NW * 32, ctas_per_sm(D, NG, GROUPED))
     total = prefix[p.S];
   }
   constexpr uint32_t CTAS = SMS * ctas_per_sm(D, NG, false);
-  const int share = GROUPED ? 1 : max(static_cast<int>((static_cast<uint32_t>(total) + CTAS - 1) / CTAS), p.min_share);
+  const int share = GROUPED ? 1 : max(static_cast<int>((static_cast<uint32_t>(total) + CTAS - 1) / CTAS), MIN_SHARE);
   const int cta = GROUPED ? blockIdx.x / CL : blockIdx.x;
   const int64_t pos0 = static_cast<int64_t>(cta) * share;
   const int end = static_cast<int>(min(pos0 + share, static_cast<int64_t>(total)));

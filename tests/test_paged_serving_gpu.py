@@ -357,6 +357,15 @@ def test_attention_wide_tables_share_the_line(seed, S, G, D):
     assert status == 0
 
 
+def test_flags_that_have_no_truth_are_refused():
+    from infercache_b200.paged_ops import page_plan, paged_attention
+    two = torch.ones(2, device="cuda")
+    with pytest.raises(RuntimeError):
+        page_plan(i32([0]), i32([1]), i32([[-1]]), i32([0]), i32([1]), 1, commit=two)
+    with pytest.raises(RuntimeError):
+        paged_attention(*attention_inputs(1, [3], [1], 1, 1, 64, torch.int8, torch.float16), return_lse=two)
+
+
 @pytest.mark.parametrize("D", [64, 128, 256])
 @pytest.mark.parametrize("G", [2, 9])
 @pytest.mark.parametrize("width", [0, 1200])
