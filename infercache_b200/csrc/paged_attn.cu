@@ -85,9 +85,12 @@ int check(const ic_paged_attn_args* a) {
 //     128 dims: 36 102 / 96, 48 103 / 95, 64 132 / 94 (40 sessions of 3000 tokens,
 //     35 rows, a second wave of tiles: 100 / 127); 256 dims: 16 117 / 164, 24 213 /
 //     165, 36 164 / 90, 64 214 / 91
+// Short tiles also want more of them, lest a long session's CTA runs alone: 24
+// sessions of 1400 tokens, 4 heads, 48 rows (4608 in all) 26 / 30 at 128 dims, 20 /
+// 26 at 64; 24 of 256 to 4096, 2 heads, 48 rows (2304) 47 / 76 at 256 dims.
 int few_rows(const ic_paged_attn_args& a) {
   const int64_t G = a.num_q_heads / a.num_kv_heads, rows = a.num_q_tokens * static_cast<int64_t>(a.num_q_heads);
-  const int few = a.head_dim == 256 ? 16 : 40;
+  const int few = a.head_dim == 256 ? (rows > 4096 ? 16 : 128) : rows > 6144 ? 40 : 64;
   return a.max_count * G <= few || rows <= (a.head_dim == 256 ? 2048 : 4096) ? ALL_ROWS : few;
 }
 
