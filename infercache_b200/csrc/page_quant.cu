@@ -9,7 +9,7 @@
 // element, a read 1 + size) as long as an element costs few instructions, which
 // is why maxima and fp16 codes are taken two at a time.  Measured (B200): 16
 // prompts of 2048 fp16 tokens, 36 layers, 2 heads, 128 dims, written as int8 and
-// read back: 600 us for 3.62 GB, 6.0 TB/s, 92 % of a plain copy's rate; one token
+// read back: 600 to 632 us for 3.62 GB, 88 to 92 % of a plain copy's rate; one token
 // of 64 sessions, 4 heads, written and read back: 8.9 us, the calls' host time.
 #include <stdio.h>
 
