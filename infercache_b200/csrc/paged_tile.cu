@@ -62,6 +62,7 @@ template <int D> constexpr int SLOTS = D == 256 ? 2 : 5;
 constexpr int NSC = 8;                 // key tiles whose scales are kept: the ring runs at most 3 ahead of the softmax
 constexpr int SORTED = 128;            // up to this many sessions are taken longest first
 constexpr float SLACK = 8.f, LIFT = 7.f;
+constexpr float MIN_FACTOR = 1.17549435e-38f;  // 2^-126
 
 template <int D>
 struct Lay {
@@ -477,6 +478,10 @@ __global__ void __launch_bounds__(THREADS, 1) tile_kernel(const Params p) {
     const int lim_all = len - n_tok + row0 / p.G + 1;         // keys that every row of the tile sees
     const uint32_t lane_off = static_cast<uint32_t>(quarter * 32) << 16;
     const uint32_t ts = tmem + lane_off, tp = tmem + lane_off + 128 + x * 64, to = tmem + lane_off + 256 + x * 128;
+    const auto factor = [&](float k) {  // a NaN softmax scale stays NaN
+      const float x = k * qmul;
+      return x < MIN_FACTOR ? MIN_FACTOR : x;
+    };
     float m_used = -INFINITY, l = 0.f;
     float sc[TB];
     bool ok = true;
@@ -493,13 +498,16 @@ __global__ void __launch_bounds__(THREADS, 1) tile_kernel(const Params p) {
 #pragma unroll
         for (int c = 0; c < TB; ++c) sc[c] = c < end ? sc[c] : -INFINITY;
       }
-      // u = s * f + lv with f > 0: a page's largest u is its largest s's
+      // u = s * f + lv with f > 0: a page's largest u is its largest s's, and a masked
+      // score stays -inf.  The product may underflow (queries of zeros, a softmax
+      // scale of 0 or near it, pages of tiny values), so it is the smallest normal
+      // number at least: scores, 2^33 at most, times 2^-126 move no weight.
       const float4* page = reinterpret_cast<const float4*>(scales + (j % NSC) * 24);
       float f[8], lv[8];
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         const float4 a = page[i], b = page[2 + i];
-        f[4 * i] = a.x * qmul; f[4 * i + 1] = a.y * qmul; f[4 * i + 2] = a.z * qmul; f[4 * i + 3] = a.w * qmul;
+        f[4 * i] = factor(a.x); f[4 * i + 1] = factor(a.y); f[4 * i + 2] = factor(a.z); f[4 * i + 3] = factor(a.w);
         lv[4 * i] = b.x; lv[4 * i + 1] = b.y; lv[4 * i + 2] = b.z; lv[4 * i + 3] = b.w;
       }
       float mx = -INFINITY;

@@ -1,0 +1,69 @@
+"""Edges of the paged serving tick on a B200: factors that vanish, indices wider
+than 32 bits, and the paths that only long rows reach.  References and bounds
+are those of paged_reference.py and test_paged_serving_gpu.py."""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+import paged_reference as ref
+from test_paged_serving_gpu import CODES, attention_inputs, check_attention, check_plan, empty_cache, gen, held, i32
+
+pytestmark = pytest.mark.gpu
+BIG = 2 ** 32
+I64 = torch.iinfo(torch.int64)
+
+
+def i64(x):
+    return torch.tensor(x, dtype=torch.int64, device="cuda")
+
+
+# ---- factors that vanish -----------------------------------------------------------
+LENS, COUNTS = [300, 200, 40], [300, 150, 3]  # 453 x 16 heads: the tile kernel's, for 64, 128 and 256 dims
+
+
+def prompt_inputs(codes, dtype, D, seed=7):
+    x = attention_inputs(seed, LENS, COUNTS, 2, 8, D, codes, dtype)
+    assert x[0].shape[0] * x[0].shape[1] > 6144
+    return x
+
+
+def check_both(x, **kw):
+    """Through the tile kernel, and with few tokens announced through the streaming kernel."""
+    for max_count in (None, 1):
+        assert check_attention(x, max_count=max_count, **kw)[2] == 0
+
+
+@pytest.mark.parametrize("codes", CODES)
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_zero_queries_over_zero_keys(codes, dtype, D):
+    """A warm-up's or a zeroed head's inputs: the first session's K and queries are
+    zero, and some queries of the others; right is the mean of the V rows seen."""
+    from infercache_b200.paged_ops import page_write
+    x = prompt_inputs(codes, dtype, D)
+    q, k, v, ks, vs, table = x[:6]
+    pages = table[0, :-(-LENS[0] // 16)].long()
+    slots = (pages[:, None] * 16 + torch.arange(16, device="cuda")).reshape(-1)[:LENS[0]]
+    keep = v.clone(), vs.clone()
+    zeros = torch.zeros(LENS[0], 2, D, device="cuda", dtype=dtype)
+    page_write(zeros, zeros, k, v, ks, vs, slots)
+    assert bool((ks[:, pages] == 2.0 ** -60).all())
+    v.view(torch.uint8).copy_(keep[0].view(torch.uint8))
+    vs.copy_(keep[1])
+    q[:LENS[0]] = 0
+    q[310:330, 3:7] = 0
+    check_both(x)
+    check_both(x, scale=1e-30)
+
+
+@pytest.mark.parametrize("codes", CODES)
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_scales_that_leave_no_score(codes, dtype, D):
+    x = prompt_inputs(codes, dtype, D)
+    check_both(x, scale=0.0)
+    check_both(((x[0] * 1e-30).to(dtype),) + x[1:], scale=1e-30)
+    tiny = x[3] * 2.0 ** -50
+    check_both(((x[0] * 1e-30).to(dtype), x[1], x[2], tiny) + x[4:], scale=-1e-20)
