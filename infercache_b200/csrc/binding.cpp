@@ -15,6 +15,7 @@
 #include <torch/csrc/utils/object_ptr.h>
 
 #include <cmath>
+#include <limits>
 #include <sstream>
 #include <string>
 
@@ -113,6 +114,8 @@ int32_t* status_word(const char* name, PyObject* o, c10::Device dev) {
 }
 
 // An int32 copy of an int32 / int64 tensor (the tensor itself when it needs none).
+// Values that 32 bits do not hold become the nearest that they do: outside every
+// pool and vocabulary, and past every length, as the value itself is.
 Tensor ints(const char* name, const char* what, const Tensor& t, c10::Device dev, at::IntArrayRef shape) {
   bool ok = (t.scalar_type() == at::kInt || t.scalar_type() == at::kLong) && t.device() == dev &&
             t.dim() == static_cast<int64_t>(shape.size());
@@ -120,7 +123,9 @@ Tensor ints(const char* name, const char* what, const Tensor& t, c10::Device dev
   if (!ok)
     bad(name, std::string(what) + " must be an int32 or int64 tensor of shape " + shape_text(shape) + " (-1: any) on " +
                   dev.str() + ", got " + c10::toString(t.scalar_type()) + " " + shape_text(t.sizes()) + " on " + t.device().str());
-  return t.scalar_type() == at::kInt ? t.contiguous() : t.to(at::kInt).contiguous();
+  if (t.scalar_type() == at::kInt) return t.contiguous();
+  using limits = std::numeric_limits<int32_t>;
+  return t.clamp(limits::min(), limits::max()).to(at::kInt).contiguous();
 }
 
 // Whether every row (last dimension) starts on a 16-byte boundary and is contiguous.

@@ -65,6 +65,8 @@ class PagedBatch:
         if isinstance(x, torch.Tensor):
             if x.shape != (self.max_sessions,) or x.dtype not in (torch.int32, torch.int64):
                 raise ValueError(f"{name} must be an int32 or int64 [{self.max_sessions}] tensor")
+            if x.dtype == torch.int64:  # more than 32 bits hold is more than any session holds
+                x = x.clamp(-2 ** 31, 2 ** 31 - 1)
             return x.to(self.device, torch.int32).contiguous()
         if len(x) != self.max_sessions:
             raise ValueError(f"{name} must have {self.max_sessions} entries, got {len(x)}")

@@ -67,3 +67,50 @@ def test_scales_that_leave_no_score(codes, dtype, D):
     check_both(((x[0] * 1e-30).to(dtype),) + x[1:], scale=1e-30)
     tiny = x[3] * 2.0 ** -50
     check_both(((x[0] * 1e-30).to(dtype), x[1], x[2], tiny) + x[4:], scale=-1e-20)
+
+
+# ---- indices wider than 32 bits ------------------------------------------------------
+OUTSIDE = [BIG, BIG + 5, -BIG + 5, I64.min, I64.max, I64.min + 3, 2 ** 31, -2 ** 31 - 1]
+
+
+@pytest.mark.parametrize("codes", CODES)
+def test_slots_beyond_32_bits_are_outside_the_pool(codes):
+    from infercache_b200.paged_ops import page_read, page_write
+    cache = [t[0] for t in empty_cache(1, 2, 3, 64, codes)]
+    x = torch.randn(1 + len(OUTSIDE), 2, 64, generator=gen(2), device="cuda").half()
+    before = [t.clone() for t in cache]
+    page_write(x[1:], x[1:], *cache, i64(OUTSIDE))
+    assert all(torch.equal(a.view(torch.uint8), b.view(torch.uint8)) for a, b in zip(cache, before))
+    page_write(x, x, *cache, i64([16] + OUTSIDE))
+    want = [t.clone() for t in before]
+    page_write(x[:1], x[:1], *want, i32([16]))
+    assert all(torch.equal(a.view(torch.uint8), b.view(torch.uint8)) for a, b in zip(cache, want))
+    k, v = page_read(*cache, i64([16] + OUTSIDE))
+    assert bool(k[:, 0].any()) and bool(v[:, 0].any()) and not k[:, 1:].any() and not v[:, 1:].any()
+
+
+def test_ids_beyond_32_bits_are_outside_the_vocabulary():
+    from infercache_b200.logits import process_logits
+    x = torch.randn(1, 200, generator=gen(3), device="cuda")
+    outside, vals = i64([OUTSIDE]), torch.ones(1, len(OUTSIDE), device="cuda")
+    got = process_logits(x, tokens=outside, repetition=3.0, presence=1.0, frequency=0.5, bias_ids=outside, bias_values=vals)
+    assert torch.equal(got, x)
+    # and lengths beyond them are all of the row
+    tok, ids = i64([[1, 2, 3, 4]]), i64([[7, 8]])
+    whole = dict(tokens=tok, repetition=3.0, frequency=1.0, bias_ids=ids, bias_values=vals[:, :2])
+    assert torch.equal(process_logits(x, **whole, token_lens=i64([BIG]), bias_lens=i64([BIG])), process_logits(x, **whole))
+    assert torch.equal(process_logits(x, **whole, prompt_lens=i64([BIG])), process_logits(x, **whole, prompt_lens=i64([4])))
+    assert torch.equal(process_logits(x, **whole, token_lens=i64([-BIG + 2])), process_logits(x, bias_ids=ids, bias_values=vals[:, :2]))
+
+
+def test_batch_counts_and_keeps_beyond_32_bits():
+    from infercache_b200 import PagedBatch
+    from test_paged_serving_gpu import make_pool
+    b = PagedBatch(make_pool(torch.int8), 4)
+    b.extend([20, 5, 1, 0])
+    b.release(i64([BIG, I64.max, I64.min, BIG + 1]))  # more than they hold, or negative: all of them
+    assert b.lens.tolist() == [20, 5, 1, 0]
+    b.extend(i64([BIG + 1, 0, -BIG + 1, 1]), total=2)  # two that cannot be had, one of them negative
+    assert b.lens.tolist()[:3] == [20, 5, 1]
+    with pytest.raises(RuntimeError):
+        b.check_device_status()
