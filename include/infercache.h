@@ -628,7 +628,7 @@ int ic_page_release(const ic_page_release_args* a, void* stream);
  * pool are skipped by a write and read as zeros), or, with slots NULL, token
  * start_token + t of the session whose pages are page_ids, as
  * ic_page_rows_args.  In a write by slots the tokens of one page stand next
- * to each other.  Element (l, h, t) of k_buf / v_buf lies at
+ * to each other and in order; slots may be left out.  Element (l, h, t) of k_buf / v_buf lies at
  * (l - layer_begin) * stride_l + h * stride_h + t * stride_t, D contiguous,
  * every such row 16-byte aligned; buf_dtype is fp32, fp16 or bf16.
  *
@@ -638,8 +638,9 @@ int ic_page_release(const ic_page_release_args* a, void* stream);
  * Codes are rounded to nearest, ties to even.  Infinities are stored as the
  * largest value, NaN as zero; both set IC_DEVFLAG_NONFINITE.
  *
- * A write of two ranges (or two runs of one range) to one page races; the
- * caller keeps them disjoint, as the allocator does.  One launch handles up
+ * Two ranges of a write must not share a page, nor must tokens of one range
+ * that another page's token or a skipped row stands between: they would race.
+ * The caller keeps them apart, as the allocator does.  One launch handles up
  * to IC_PAGE_BATCH_MAX ranges (`rows` is host memory, copied at the call). */
 typedef struct ic_page_q8_rows {
   const int32_t* slots;

@@ -1,7 +1,7 @@
 // Rows into and out of 8-bit pages.
 //
 // Write: one warp per (page run, layer and head, K or V) -- a run is the
-// tokens of one call that land in one page.  The run's rows pass through a few
+// tokens of one call that land in one page, one after another.  The run's rows pass through a few
 // vectors per lane: their largest magnitude gives the page scale's exponent, then
 // the codes are stored; a run that does not start its page and needs a larger
 // scale first rounds the page's other codes again.  Read: one thread per
@@ -41,7 +41,7 @@ struct Batch {
   int32_t* status;
   int64_t pool_tokens;
   int32_t heads, layer_begin, count;
-  int32_t window;                        // slots form of a write: tokens whose runs one warp looks after
+  int32_t window;                        // slots form of a write: tokens whose pages one warp looks after
   int64_t first[IC_PAGE_BATCH_MAX + 1];  // work items (warps or threads) before each range
   Range r[IC_PAGE_BATCH_MAX];
 };
@@ -284,26 +284,30 @@ __global__ void __launch_bounds__(WARPS * 32, 8) write_kernel(const __grid_const
                           scales + slot / q8::PAGE, b.status, lane);
     return;
   }
-  // the runs that begin among tokens w0 .. w0 + window - 1 (window <= 16):
-  // lane j holds token w0 - 1 + j's slot
+  // the pages whose first token is among tokens w0 .. w0 + window - 1 (window <=
+  // 16): lane j holds token w0 - 1 + j's slot.  A page's tokens are one warp's, run
+  // after run where they leave slots out: two runs raise one scale.
   const int64_t w0 = w * b.window, tj = w0 - 1 + lane;
   const int32_t slot = tj >= 0 && tj < r.n ? r.slots[tj] : -1;
   const int32_t prev = __shfl_up_sync(FULL_MASK, slot, 1);
   const bool valid = slot >= 0 && slot < b.pool_tokens;
-  // a run goes on while the next token takes the next slot of the same page
-  const bool follows = lane > 0 && valid && prev >= 0 && slot == prev + 1 && slot % q8::PAGE != 0;
-  const uint32_t cont = __ballot_sync(FULL_MASK, follows);
-  uint32_t heads = __ballot_sync(FULL_MASK, valid && !follows && lane >= 1 && lane <= b.window);
+  const bool same = lane > 0 && valid && prev >= 0 && slot / q8::PAGE == prev / q8::PAGE;
+  const uint32_t page_goes_on = __ballot_sync(FULL_MASK, same);
+  const uint32_t cont = __ballot_sync(FULL_MASK, same && slot == prev + 1);  // the next slot: the same run
+  uint32_t heads = __ballot_sync(FULL_MASK, valid && !same && lane >= 1 && lane <= b.window);
   while (heads) {
-    const int j = __ffs(heads) - 1;
+    int j = __ffs(heads) - 1;
     heads &= heads - 1;
-    const int32_t s0 = __shfl_sync(FULL_MASK, slot, j);
-    const uint32_t rest = ~(cont >> j >> 1);  // bit k: token j + 1 + k does not go on
-    const int cnt = min(__ffs(rest), q8::PAGE - s0 % q8::PAGE);
-    write_run<T, D, CODE, CHUNK>(buf + (w0 - 1 + j) * r.stride_t, r.stride_t, cnt, s0 % q8::PAGE,
-                          codes + static_cast<int64_t>(s0 / q8::PAGE) * (q8::PAGE * D), scales + s0 / q8::PAGE, b.status,
-                          lane);
-    __syncwarp();
+    do {
+      const int32_t s0 = __shfl_sync(FULL_MASK, slot, j);
+      const uint32_t rest = ~(cont >> j >> 1);  // bit k: token j + 1 + k does not go on
+      const int cnt = min(__ffs(rest), q8::PAGE - s0 % q8::PAGE);
+      write_run<T, D, CODE, CHUNK>(buf + (w0 - 1 + j) * r.stride_t, r.stride_t, cnt, s0 % q8::PAGE,
+                            codes + static_cast<int64_t>(s0 / q8::PAGE) * (q8::PAGE * D), scales + s0 / q8::PAGE, b.status,
+                            lane);
+      __syncwarp();
+      j += cnt;
+    } while (j < 32 && (page_goes_on >> j & 1));
   }
 }
 
@@ -478,7 +482,7 @@ extern "C" int ic_page_write_q8(const ic_page_q8_args* a, void* stream) {
   if (planes == 0) return IC_OK;
   Batch b = {};
   fill_batch(a, b);
-  // Slots form: a warp looks after the runs that begin among `window` tokens.
+  // Slots form: a warp looks after the pages whose first token is among `window` tokens.
   // One while that leaves few warps (a decode tick: every run is one token and
   // all run side by side); with many, 4 and then 16, so that a prompt's warps
   // have a page each instead of most of them finding nothing to do.

@@ -84,8 +84,9 @@ def page_write(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache:
     ``k``, ``v`` [N, H, D] into a cache [H, pool_tokens, D], or [L, N, H, D] into
     [L, H, pool_tokens, D]; fp32, fp16 or bf16, any strides (rows that are not
     contiguous and 16-byte aligned are copied first).  Token i goes to pool row
-    ``slots[i]``; the tokens of one page stand next to each other and in order, no
-    row occurs twice, and rows outside the pool are skipped.  A page is written
+    ``slots[i]``; the tokens of one page stand next to each other and in order (slots
+    may be left out), no row occurs twice, and rows outside the pool are skipped
+    (not from among a page's tokens).  A page is written
     in order: tokens that begin at its slot 0 start it anew, later ones keep its
     scale or raise it (the page's other codes are then rounded again).
     Infinities are stored as the largest value and NaN as zero; both set

@@ -114,3 +114,34 @@ def test_batch_counts_and_keeps_beyond_32_bits():
     assert b.lens.tolist()[:3] == [20, 5, 1]
     with pytest.raises(RuntimeError):
         b.check_device_status()
+
+
+# ---- pages whose tokens leave slots out ------------------------------------------------
+@pytest.mark.parametrize("codes", CODES)
+@pytest.mark.parametrize("pages,H", [(60, 2), (500, 4), (1400, 8)])
+def test_write_leaves_slots_out(codes, pages, H):
+    """A page's tokens in order but not in consecutive slots are one warp's, run
+    after run: the scale covers them all.  Sizes at which a warp looks after 1, 4
+    and 16 tokens."""
+    from infercache_b200.paged_ops import page_write
+    rng = np.random.default_rng(pages)
+    slots = []
+    for page in rng.permutation(pages + 20)[:pages].tolist():
+        slots += [page * 16 + j for j in range(16) if rng.random() < 0.45]
+    n = len(slots) * H
+    assert n <= 8192 if pages == 60 else 8192 < n <= 65536 if pages == 500 else n > 65536
+    cache = [t[0] for t in empty_cache(1, H, pages + 20, 64, codes, 1)]
+    planes = [(c, s, np.nan_to_num(held(c, s)), s.cpu().double().numpy().copy()) for c, s in zip(cache[:2], cache[2:])]
+    g, known = gen(2), set()
+    for piece, scale in ((slots, 1.0), ([5, 7, 9, 15], 6.0), ([48, 50], 0.5), ([20, 22, 23, 31], 40.0)):
+        new = [(torch.randn(len(piece), H, 64, generator=g, device="cuda") * scale).bfloat16() for _ in range(2)]
+        page_write(*new, *cache, i32(piece))
+        anew = {x // 16 for x in piece if x % 16 == 0}  # what stood in these pages is gone
+        known = {x for x in known if x // 16 not in anew} | set(piece)
+        at, held_pages = sorted(known), sorted({x // 16 for x in known})
+        for x, (c, s, want, wscale) in zip(new, planes):
+            rows = x.double().cpu().numpy()
+            for h in range(H):
+                ref.write(want[h], wscale[h], rows[:, h], piece, codes)
+            assert np.array_equal(held(c, s)[:, at], want[:, at])
+            assert np.array_equal(s.cpu().double().numpy()[:, held_pages], wscale[:, held_pages])
