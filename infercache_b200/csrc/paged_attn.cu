@@ -59,12 +59,20 @@ int check(const ic_paged_attn_args* a) {
     set_last_error("paged_attention: at most 4096 sessions");
     return IC_ERR_UNSUPPORTED;
   }
-  // the streaming kernel numbers all groups' pages, and its overhead for each
-  // group, with 32 bits
-  const int64_t G = a->num_q_heads / a->num_kv_heads;
-  const int64_t tiles = a->num_q_tokens * G / 8 + a->num_sessions;
+  // The tile kernel's grid and a session's rows fit 31 bits.
+  const int64_t G = a->num_q_heads / a->num_kv_heads, rows = a->num_q_tokens * G;
+  if (rows > (1 << 30) || (rows / 128 + a->num_sessions) * a->num_kv_heads > 0x7fffffff) {
+    set_last_error("paged_attention: more than 2^30 query rows per KV head, or 2^31 tiles of them in all");
+    return IC_ERR_UNSUPPORTED;
+  }
+  // The streaming kernel numbers its groups' pages, and its overhead for each
+  // group, with 32 bits.  Its groups: tiles of 8 rows or more, and no more than
+  // few_rows of a session where the tile kernel has the others.
+  const int few = few_rows(*a);
+  int64_t tiles = rows / 8 + a->num_sessions;
+  if (few != ALL_ROWS) tiles = std::min(tiles, static_cast<int64_t>(a->num_sessions) * ((few + 7) / 8));
   if (tiles * a->num_kv_heads > 0x7fffffffLL / (a->table_width + 32)) {
-    set_last_error("paged_attention: query tiles x KV heads x table width exceed 2^31");
+    set_last_error("paged_attention: the streaming kernel's query tiles x KV heads x table width exceed 2^31");
     return IC_ERR_UNSUPPORTED;
   }
   return IC_OK;

@@ -20,3 +20,32 @@ def test_smoke_as_a_script_finds_every_part():
     guard = [i for i, x in enumerate(body) if isinstance(x, ast.If)]
     defs = [i for i, x in enumerate(body) if isinstance(x, ast.FunctionDef)]
     assert len(guard) == 1 and guard[0] > max(defs)
+
+
+def attention_args(**kw):
+    import ctypes
+    from infercache_b200 import _lib
+    buf = ctypes.create_string_buffer(64)
+    p = (ctypes.addressof(buf) + 15) // 16 * 16  # never read: the workspace's size alone is asked for
+    base = dict(q=p, out=p, k=p, v=p, k_scale=p, v_scale=p, block_table=p, lens=p, q_start=p, pool_tokens=2 ** 20,
+                q_stride_t=4096, q_stride_h=128, num_sessions=1, table_width=8192, num_q_heads=32, num_kv_heads=8, head_dim=128,
+                q_dtype=_lib.IC_F16, code_dtype=_lib.IC_E4M3, scale=0.1)
+    base.update(kw)
+    base.setdefault("max_count", base["num_q_tokens"])
+    return _lib.ic_paged_attn_args(**base)
+
+
+def attention_takes(**kw):
+    import ctypes
+    from infercache_b200 import _lib
+    return _lib.load().ic_paged_attention_workspace(ctypes.byref(attention_args(**kw))) > 0
+
+
+def test_attention_takes_long_prompts_under_wide_tables():
+    """The table's width bounds the streaming kernel's work, not the tile kernel's."""
+    assert attention_takes(num_q_tokens=65_300)
+    assert attention_takes(num_q_tokens=131_072, head_dim=256)
+    assert attention_takes(num_q_tokens=200_000, num_sessions=64, max_count=130_000)
+    assert not attention_takes(num_q_tokens=65_300, max_count=1)               # all of it the streaming kernel's
+    assert not attention_takes(num_q_tokens=2 ** 29)                           # 2^31 rows per KV head
+    assert not attention_takes(num_q_tokens=2 ** 26, num_q_heads=8192, num_kv_heads=8192, table_width=64)

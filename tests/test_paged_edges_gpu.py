@@ -145,3 +145,23 @@ def test_write_leaves_slots_out(codes, pages, H):
                 ref.write(want[h], wscale[h], rows[:, h], piece, codes)
             assert np.array_equal(held(c, s)[:, at], want[:, at])
             assert np.array_equal(s.cpu().double().numpy()[:, held_pages], wscale[:, held_pages])
+
+
+# ---- one long prompt in one call -----------------------------------------------------
+def test_long_prompt_with_a_wide_table():
+    """65.3k tokens x 8 KV heads of 4 under a table for 128k tokens: the tile
+    kernel's, whose work the table's width does not bound."""
+    from infercache_b200.paged_ops import paged_attention
+    n, H, G, D, width = 65_300, 8, 4, 64, 8192
+    x = list(attention_inputs(5, [n], [n], H, G, D, torch.int8, torch.float16))
+    wide = torch.full((1, width), -1, dtype=torch.int32, device="cuda")
+    wide[:, :x[5].shape[1]] = x[5]
+    x[5] = wide
+    out, lse = paged_attention(*x, return_lse=True)
+    at = [0, 1, 15, 16, 127, 128, 129, 5000, 33_333, 65_298, 65_299]
+    q, k, v, ks, vs = x[:5]
+    # a query's row is that of a session that ends with it
+    want, wlse, tol, ltol = ref.attention(q[at], ref.cache_values(k, ks), ref.cache_values(v, vs), wide.expand(len(at), width),
+                                          [i + 1 for i in at], list(range(len(at) + 1)), D ** -0.5)
+    assert float(((out[at].double() - want).abs() - tol).max()) <= 0
+    assert float(((lse[at].double() - wlse).abs() - ltol).max()) <= 0
