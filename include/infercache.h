@@ -574,7 +574,8 @@ int ic_graph_select(const ic_graph_select_args* a, void* stream);
  *   q_start[s]       exclusive prefix sum of counts, S + 1 entries (negative
  *                    counts count as 0)
  *   slots[i]         pool row (page * 16 + slot) of new token i, -1 for a
- *                    denied session's tokens and for i >= q_start[S]
+ *                    denied session's tokens, for i >= q_start[S] and where
+ *                    the page id is negative or 2^27 and more (no pool's)
  *   positions[i]     its position in its session, -1 likewise
  *   lens_out[s]      lens[s] + counts[s], or lens[s] when denied
  *   *free_count_out  what is left of the stack

@@ -52,6 +52,11 @@ __device__ __forceinline__ int64_t block_scan(int64_t v, int64_t* warp_sums, int
   return v + (warp > 0 ? before : 0);
 }
 
+// Pool row of a page's slot; -1 for a page that no pool has (its rows fit 31 bits).
+__device__ __forceinline__ int32_t row_of(int32_t page, int32_t slot) {
+  return static_cast<uint32_t>(page) > 0x7fffffffu / q8::PAGE ? -1 : page * q8::PAGE + slot;
+}
+
 __device__ __forceinline__ int32_t pages_of(int64_t tokens) {
   return static_cast<int32_t>((tokens + q8::PAGE - 1) / q8::PAGE);
 }
@@ -103,7 +108,7 @@ __device__ __forceinline__ void plan_tokens(const ic_page_plan_args& a, const in
         for (int k = 0; k < 2; ++k) {
           const uint32_t p = p0 + 64 * (j >> 1) + k;
           if (p % q8::PAGE == 0 && p / q8::PAGE >= held) row[p / q8::PAGE] = page[j + k];
-          slot[k] = page[j + k] < 0 ? -1 : page[j + k] * q8::PAGE + static_cast<int32_t>(p % q8::PAGE);
+          slot[k] = row_of(page[j + k], static_cast<int32_t>(p % q8::PAGE));
         }
         const int64_t i = i0 + 64 * (j >> 1) + 2 * lane, p = p0 + 64 * (j >> 1);
         *reinterpret_cast<int2*>(a.slots + i) = make_int2(slot[0], slot[1]);
@@ -136,7 +141,7 @@ __device__ __forceinline__ void plan_tokens(const ic_page_plan_args& a, const in
         int32_t* row = a.block_table + static_cast<int64_t>(x) * a.width;
         const int32_t page = idx < held ? row[idx] : a.free_pages[top - 1 - (rank_of(x) + idx - held)];
         if (idx >= held && pos % q8::PAGE == 0) row[idx] = page;  // a new page's first token enters it
-        slot = page < 0 ? -1 : page * q8::PAGE + pos % q8::PAGE;
+        slot = row_of(page, pos % q8::PAGE);
       }
       a.slots[i] = slot;
       a.positions[i] = pos;

@@ -165,3 +165,24 @@ def test_long_prompt_with_a_wide_table():
                                           [i + 1 for i in at], list(range(len(at) + 1)), D ** -0.5)
     assert float(((out[at].double() - want).abs() - tol).max()) <= 0
     assert float(((lse[at].double() - wlse).abs() - ltol).max()) <= 0
+
+
+# ---- page ids no pool has --------------------------------------------------------------
+@pytest.mark.parametrize("S,count", [(3, 40), (40, 2000)])
+def test_plan_gives_no_slot_for_page_ids_past_32_bit_rows(S, count):
+    """Ids from 2^27 on, whose rows would not fit 32 bits, are no pool's: slot -1, as
+    for negative ones, through the one-kernel plan and the two-kernel one."""
+    from infercache_b200.paged_ops import page_plan
+    need = -(-count // 16)
+    ids = list(range(S * need))
+    for i, bad in ((1, 2 ** 27), (4, 2 ** 31 - 1), (7, -5), (2 * need + 1, 2 ** 28 + 3)):
+        ids[i] = bad
+    ids[0] = 2 ** 27 - 1  # the last that fits
+    table = i32([[-1] * need] * S)
+    p = page_plan(i32([0] * S), i32([count] * S), table, i32(ids), i32([len(ids)]), S * count, max_count=count)
+    want = []
+    for s in range(S):
+        for t in range(count):
+            page = ids[len(ids) - 1 - s * need - t // 16]
+            want.append(page * 16 + t % 16 if 0 <= page < 2 ** 27 else -1)
+    assert p.slots.tolist() == want
