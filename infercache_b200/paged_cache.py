@@ -166,9 +166,11 @@ class PagePool:
         return page_id * PAGE_SIZE + slot
 
     def _page_ids(self, page_ids) -> torch.Tensor:
-        """int32 page ids on the pool's device (a device tensor passes through)."""
+        """int32 page ids on the pool's device (such a tensor passes through)."""
         if isinstance(page_ids, torch.Tensor):
-            return page_ids
+            if page_ids.dtype == torch.int64:  # no pool has a page that 32 bits do not hold
+                page_ids = page_ids.clamp(-2 ** 31, 2 ** 31 - 1)
+            return page_ids.to(self.device, torch.int32).contiguous()
         return torch.tensor(page_ids, dtype=torch.int32).to(self.device, non_blocking=True)
 
     def write_rows(self, page_ids: List[int], start_token: int, k: torch.Tensor, v: torch.Tensor,

@@ -49,3 +49,17 @@ def test_attention_takes_long_prompts_under_wide_tables():
     assert not attention_takes(num_q_tokens=65_300, max_count=1)               # all of it the streaming kernel's
     assert not attention_takes(num_q_tokens=2 ** 29)                           # 2^31 rows per KV head
     assert not attention_takes(num_q_tokens=2 ** 26, num_q_heads=8192, num_kv_heads=8192, table_width=64)
+
+
+def test_page_ids_reach_the_kernels_as_int32_on_the_pools_device():
+    """A host or int64 tensor's address would be read as if it were neither."""
+    from infercache_b200 import PagePool
+    pool = PagePool.__new__(PagePool)
+    pool.K = torch.empty(0, device="meta")
+    ready = torch.empty(4, dtype=torch.int32, device="meta")
+    assert pool._page_ids(ready) is ready
+    for ids in (torch.arange(4), torch.arange(4, dtype=torch.int32), ready.long(), ready[::2], [1, 2, 3]):
+        got = pool._page_ids(ids)
+        assert got.dtype == torch.int32 and got.device == pool.device and got.is_contiguous()
+    pool.K = torch.empty(0)
+    assert pool._page_ids(torch.tensor([3, 2 ** 32 + 1, -2 ** 40])).tolist() == [3, 2 ** 31 - 1, -2 ** 31]
