@@ -327,10 +327,14 @@ def binding():
     if _BINDING is None:
         load()
         if not BINDING_PATH.exists():
-            raise ImportError(f"{BINDING_PATH} is missing: run `python -m infercache_b200.build`")
+            raise ImportError(f"{BINDING_PATH} is missing: run `python -m infercache_b200.build` "
+                              "(it says so when torch or Python's headers do not allow it)")
         spec = importlib.util.spec_from_file_location("infercache_b200._binding", BINDING_PATH)
         module = importlib.util.module_from_spec(spec)
         spec.loader.exec_module(module)
+        if module.torch_version != torch.__version__:
+            raise ImportError(f"{BINDING_PATH} was built for torch {module.torch_version}, this is {torch.__version__}: "
+                              "run `python -m infercache_b200.build`")
         module.setup(require_device, raise_for)
         _BINDING = module
     return _BINDING

@@ -7,7 +7,8 @@ machine without a GPU) and links ``lib/libinfercache_b200.so`` with the CUDA
 runtime linked statically, so the library does not depend on which
 libcudart the host process loaded first.  Then compiles ``csrc/binding.cpp``
 (the paged serving tick's calls on torch tensors) with g++ against the torch
-that runs this, as ``lib/_binding.so``.
+that runs this, as ``lib/_binding.so``; without a CUDA build of torch or
+Python's headers the library is built alone.
 """
 from __future__ import annotations
 
@@ -18,6 +19,7 @@ import shutil
 import subprocess
 import sys
 from pathlib import Path
+from typing import Optional
 
 PKG = Path(__file__).resolve().parent
 ROOT = PKG.parent
@@ -80,24 +82,51 @@ def build(force: bool = False, verbose: bool = False) -> Path:
     return LIB
 
 
-def build_binding(force: bool = False) -> Path:
-    src = CSRC / "binding.cpp"
-    if not force and not _stale(BINDING, [src, ROOT / "include" / "infercache.h"]):
-        return BINDING
+def _python_include() -> Path:
     import sysconfig
+    return Path(sysconfig.get_paths()["include"])
 
+
+def _no_binding() -> str:
+    """Why the binding cannot be built here ('' when it can)."""
+    import torch
+    if torch.version.cuda is None:
+        return f"torch {torch.__version__} is not a CUDA build"
+    if not (_python_include() / "Python.h").exists():
+        return f"Python's headers are not in {_python_include()}"
+    if not shutil.which("g++"):
+        return "g++ not found"
+    return ""
+
+
+def build_binding(force: bool = False) -> Optional[Path]:
+    """The binding, or None, with a line on stderr, where torch, Python's headers
+    or g++ do not allow it; the C-ABI library does not need them."""
+    why = _no_binding()
+    if why:
+        sys.stderr.write(f"the paged serving tick's binding is not built: {why}\n")
+        return None
     import torch
     from torch.utils.cpp_extension import include_paths, library_paths
-    inc = include_paths() + [sysconfig.get_paths()["include"], str(Path(nvcc()).resolve().parents[1] / "include")]
-    cmd = [shutil.which("g++") or "g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
-           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}", *(f"-I{d}" for d in inc), str(src),
+    src = CSRC / "binding.cpp"
+    cmd = [shutil.which("g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}", f'-DIC_TORCH_VERSION="{torch.__version__}"',
+           *(f"-I{d}" for d in [*include_paths(), _python_include(), Path(nvcc()).resolve().parents[1] / "include"]), str(src),
            "-o", str(BINDING), f"-L{LIBDIR}", "-linfercache_b200", "-Wl,-rpath,$ORIGIN",
            *(f"-L{d}" for d in library_paths()), *(f"-Wl,-rpath,{d}" for d in library_paths()),
            "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_cuda", "-ltorch_python"]
+    # the command names the torch, Python and compiler that it is built for: with
+    # others it is another one
+    OBJ.mkdir(exist_ok=True)
+    made_by = OBJ / "binding.cmd"
+    if (not force and not _stale(BINDING, [src, ROOT / "include" / "infercache.h"]) and made_by.exists()
+            and made_by.read_text() == "\n".join(cmd)):
+        return BINDING
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:
         sys.stderr.write(r.stdout + r.stderr)
         raise RuntimeError("g++ failed on binding.cpp")
+    made_by.write_text("\n".join(cmd))
     return BINDING
 
 

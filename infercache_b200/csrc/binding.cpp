@@ -572,4 +572,9 @@ PyModuleDef module = {PyModuleDef_HEAD_INIT, "_binding", nullptr, -1, methods, n
 
 }  // namespace
 
-PyMODINIT_FUNC PyInit__binding(void) { return PyModule_Create(&module); }
+PyMODINIT_FUNC PyInit__binding(void) {
+  PyObject* m = PyModule_Create(&module);
+  // torch's C++ interface differs from version to version: the loader compares
+  if (m && PyModule_AddStringConstant(m, "torch_version", IC_TORCH_VERSION) < 0) Py_CLEAR(m);
+  return m;
+}

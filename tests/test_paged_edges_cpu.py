@@ -1,4 +1,5 @@
 """Edges of the paged serving tick that show without a GPU."""
+import pytest
 import torch
 
 
@@ -63,3 +64,37 @@ def test_page_ids_reach_the_kernels_as_int32_on_the_pools_device():
         assert got.dtype == torch.int32 and got.device == pool.device and got.is_contiguous()
     pool.K = torch.empty(0)
     assert pool._page_ids(torch.tensor([3, 2 ** 32 + 1, -2 ** 40])).tolist() == [3, 2 ** 31 - 1, -2 ** 31]
+
+
+@pytest.mark.parametrize("missing", ["cuda", "headers"])
+def test_library_builds_without_what_the_binding_needs(missing, monkeypatch, capsys):
+    from pathlib import Path
+    from infercache_b200 import build
+    before = build.BINDING.stat().st_mtime_ns
+    if missing == "cuda":
+        monkeypatch.setattr(torch.version, "cuda", None)
+    else:
+        monkeypatch.setattr(build, "_python_include", lambda: Path("/nonexistent"))
+    assert build.build() == build.LIB
+    assert "binding is not built" in capsys.readouterr().err
+    assert build.BINDING.stat().st_mtime_ns == before
+
+
+def test_binding_is_rebuilt_for_another_torch(monkeypatch):
+    from infercache_b200 import _lib, build
+    build.build()
+    ran = []
+
+    class Done:
+        returncode = 1
+        stdout = stderr = ""
+
+    monkeypatch.setattr(build.subprocess, "run", lambda cmd, **kw: ran.append(cmd) or Done)
+    assert build.build_binding() == build.BINDING and not ran
+    monkeypatch.setattr(torch, "__version__", "9.9.9")
+    with pytest.raises(RuntimeError):  # it set out to compile
+        build.build_binding()
+    assert len(ran) == 1
+    monkeypatch.setattr(_lib, "_BINDING", None)
+    with pytest.raises(ImportError, match="9.9.9"):
+        _lib.binding()
