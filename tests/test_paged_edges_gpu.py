@@ -186,3 +186,91 @@ def test_plan_gives_no_slot_for_page_ids_past_32_bit_rows(S, count):
             page = ids[len(ids) - 1 - s * need - t // 16]
             want.append(page * 16 + t % 16 if 0 <= page < 2 ** 27 else -1)
     assert p.slots.tolist() == want
+
+
+# ---- logits rows longer than the kernel's first reach ----------------------------------
+def check_long_logits(V, S, T, B, dtype, spread, seed, in_place):
+    from infercache_b200.logits import process_logits
+    rng = np.random.default_rng(seed)
+    x = torch.randn(S, V, generator=gen(seed), device="cuda").mul(3).to(dtype)
+    kw, lens, prompt, bias = {}, [0] * S, [0] * S, [{}] * S
+    tokens = np.zeros((S, max(T, 1)), np.int64)
+    rep, pres, freq = [1.3, 0.7][:S], [0.5, -0.25][:S], [0.001, 0.003][:S]
+    if T:
+        tokens = rng.integers(0, spread, (S, T))
+        tokens[:, ::11] = rng.integers(-3, V + 3, tokens[:, ::11].shape)
+        lens, prompt = [T, T - 7][:S], [T // 3, 5][:S]
+        kw.update(tokens=torch.from_numpy(tokens).cuda().int(), token_lens=i32(lens), prompt_lens=i32(prompt),
+                  repetition=torch.tensor(rep, device="cuda"), presence=torch.tensor(pres, device="cuda"),
+                  frequency=torch.tensor(freq, device="cuda"))
+    if B:
+        ids, vals = rng.integers(-3, V + 3, (S, B)), rng.normal(size=(S, B)).astype(np.float32)
+        ids[:, B // 2:B // 2 + 20] = ids[:, :20]  # given twice: the last value counts
+        blens = [B, B - 3][:S]
+        bias = [dict(zip(ids[r, :blens[r]].tolist(), vals[r, :blens[r]].tolist())) for r in range(S)]
+        kw.update(bias_ids=i32(ids), bias_values=torch.from_numpy(vals).cuda(), bias_lens=i32(blens))
+    f32 = lambda v: [float(np.float32(a)) for a in v]  # noqa: E731
+    want = ref.logits(x.cpu(), tokens, lens, prompt, f32(rep), f32(pres), f32(freq), bias, None)
+    # the penalty's product (two roundings), the term of count and presence (two), a
+    # difference and a sum: each at most half a step of the largest intermediate
+    n = max(np.bincount(np.clip(tokens[r], 0, V)).max() for r in range(S)) if T else 0
+    tol = 6 * 2.0 ** -24 * (2 * x.cpu().double().abs() + float(n) * 0.003 + 1 + 6)
+    got = process_logits(x, **kw, **(dict(out=x) if in_place else {})).cpu().double()
+    assert bool(((got - want).abs() <= tol).all())
+
+
+@pytest.mark.parametrize("in_place", [False, True])
+@pytest.mark.parametrize("V", [8192, 32001])
+@pytest.mark.parametrize("T,B", [(5000, 0), (5000, 40), (2049, 3000), (0, 5000), (70000, 0), (70000, 40), (50, 33000), (0, 33000),
+                                 (70000, 33000)])
+def test_logits_long_rows(V, T, B, in_place):
+    """Past 2048 tokens, past the list of 2048 named ids, past 65535 tokens and 32766
+    biases, each with and without the other part."""
+    check_long_logits(V, 2, T, B, torch.float32, V, T + B, in_place)
+
+
+@pytest.mark.parametrize("T,B,spread", [(5000, 0, 6000), (5000, 300, 8192), (70000, 0, 8000), (70000, 33000, 8192)])
+def test_logits_long_rows_in_one_large_chunk(T, B, spread):
+    """A batch large enough for chunks of 8192 ids, most of whose first chunk is named."""
+    check_long_logits(8192 * 700, 1, T, B, torch.bfloat16, spread, 3, False)
+
+
+# ---- calls the documentation allows ------------------------------------------------------
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("max_count", [1, None])
+def test_attention_writes_over_its_queries(D, max_count):
+    """out may be q: a row is read by those alone that write it, before they do;
+    one long session in shares, and many rows in tiles."""
+    from infercache_b200.paged_ops import paged_attention
+    for lens, counts in (([20000, 90], [2, 1]), (LENS, COUNTS)):
+        x = attention_inputs(D, lens, counts, 2, 8, D, CODES[0], torch.float16)
+        want = paged_attention(*x, max_count=max_count)
+        q = x[0].clone()
+        got = paged_attention(q, *x[1:], max_count=max_count, out=q)
+        assert got is q and torch.equal(q, want)
+
+
+@pytest.mark.parametrize("max_count", [1, None])
+def test_attention_rows_before_the_first_session(max_count):
+    from infercache_b200.paged_ops import paged_attention
+    x = attention_inputs(4, LENS, COUNTS, 2, 8, 128, CODES[1], torch.bfloat16)
+    want, wlse = paged_attention(*x, max_count=max_count, return_lse=True)
+    q = torch.cat([torch.full((5, 16, 128), math.nan, device="cuda").bfloat16(), x[0]])
+    out = torch.full_like(q, 9.0)
+    got, lse = paged_attention(q, *x[1:7], x[7] + 5, max_count=max_count, out=out, return_lse=True)
+    assert bool((out[:5] == 9).all()) and torch.equal(out[5:], want) and torch.equal(lse[5:], wlse)
+
+
+@pytest.mark.parametrize("S", [31, 32, 33, 127, 128, 129])
+def test_attention_numbers_of_sessions(S):
+    """Around the counts where the kernels look sessions up in another way, alone and
+    with one session's prompt beside them."""
+    rng = np.random.default_rng(S)
+    lens = rng.integers(0, 200, S).tolist()
+    counts = [min(n, int(c)) for n, c in zip(lens, rng.integers(0, 3, S))]
+    lens[-1] = counts[-1] = 1
+    check_attention(attention_inputs(S, lens, counts, 2, 4, 64, CODES[S % 2], torch.float16), max_count=2)
+    lens[S // 2], counts[S // 2] = 900, 850
+    x = attention_inputs(S, lens, counts, 2, 4, 64, CODES[S % 2], torch.float16)
+    assert x[0].shape[0] * x[0].shape[1] > 6144
+    check_attention(x)
