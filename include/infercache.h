@@ -717,8 +717,9 @@ int64_t ic_paged_attention_workspace(const ic_paged_attn_args* a);
 /* ---- Penalties, biases and grammar masks on logits --------------------------------
  * For every row r and id v, in 32 bits:
  *   x = logits[r, v]
- *   x = x > 0 ? x * (1 / repetition[r]) : x * repetition[r]
+ *   x = x > 0 ? x / repetition[r] : x * repetition[r]
  *                                     if v is among tokens[r, 0 .. token_lens[r])
+ *                                     (for repetition_all: x * repetition_all_inv)
  *   x = x - (frequency[r] * n + presence[r] * (n > 0))
  *                                     n = how often v is among tokens[r,
  *                                     prompt_lens[r] .. token_lens[r])

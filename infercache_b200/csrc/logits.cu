@@ -169,7 +169,6 @@ __global__ void __launch_bounds__(LT) logits_kernel(const ic_logits_args a) {
 
   // ---- the ids that are named ---------------------------------------------------
   const float rep = a.repetition ? a.repetition[row] : a.repetition_all;
-  const float inv_rep = a.repetition ? 1.f / rep : a.repetition_all_inv;
   const float freq = a.frequency ? a.frequency[row] : a.frequency_all;
   const float pres = a.presence ? a.presence[row] : a.presence_all;
   const float* bias = a.bias_values + row * a.bias_stride;
@@ -180,7 +179,9 @@ __global__ void __launch_bounds__(LT) logits_kernel(const ic_logits_args a) {
     float x = DT<T>::to_f(in[rel]);
     const uint32_t c = w & COUNT;
     if (c != 0 || (w & SEEN)) {
-      x = x > 0.f ? x * inv_rep : x * rep;
+      // a row's own penalty divides, rounding once; a number's reciprocal comes from
+      // the caller, as torch divides by a number
+      x = !(x > 0.f) ? x * rep : a.repetition ? __fdiv_rn(x, rep) : x * a.repetition_all_inv;
       if (c != 0) x = __fsub_rn(x, __fadd_rn(__fmul_rn(freq, static_cast<float>(c)), pres));
     }
     if (b != 0) x += bias[b - 1];

@@ -25,7 +25,8 @@ def process_logits(logits: torch.Tensor, *, tokens: Optional[torch.Tensor] = Non
     """float32 logits [S, V] after, in this order,
 
     * ``repetition`` r: an id among ``tokens[s, :token_lens[s]]`` (prompt and
-      answer) has x * (1 / r) where x > 0, x * r elsewhere;
+      answer) has x / r where x > 0 (x * (1 / r) for a number r, as torch
+      divides by a number), x * r elsewhere;
     * ``frequency`` f and ``presence`` p: x - (f * n + p) for an id that occurs
       n > 0 times in the answer, ``tokens[s, prompt_lens[s]:token_lens[s]]``;
     * ``bias_ids`` / ``bias_values`` [S, B] (the first ``bias_lens[s]`` of a row):

@@ -274,3 +274,18 @@ def test_attention_numbers_of_sessions(S):
     x = attention_inputs(S, lens, counts, 2, 4, 64, CODES[S % 2], torch.float16)
     assert x[0].shape[0] * x[0].shape[1] > 6144
     check_attention(x)
+
+
+# ---- roundings of the repetition penalty --------------------------------------------------
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_rows_own_repetition_penalty_rounds_once(dtype):
+    """x / r as 32 bits give it, bit for bit, where r is the row's; NaN, infinities
+    and zeros as the comparison sends them."""
+    from infercache_b200.logits import process_logits
+    x = (torch.randn(6, 20000, generator=gen(8), device="cuda") * 5).to(dtype)
+    x[:, :5] = torch.tensor([math.nan, math.inf, -math.inf, 0.0, -0.0], device="cuda").to(dtype)
+    r = torch.tensor([1.1, 1.3, 0.9, 3.0, 1.7, 1e-3], device="cuda")
+    said = torch.arange(0, 20000, device="cuda", dtype=torch.int32).expand(6, -1)
+    f = x.float()
+    want = torch.where(f > 0, f / r[:, None], f * r[:, None])
+    assert torch.equal(process_logits(x, tokens=said, repetition=r).view(torch.int32), want.view(torch.int32))
