@@ -607,7 +607,8 @@ int ic_page_plan(const ic_page_plan_args* a, void* stream);
  * lens[s] or keep[s] < 0; none when keep[s] = 0, the end of a request): the
  * pages behind them go back on the stack, in session and page order from the
  * top, so that the next plan hands them out in that order; their table entries
- * become -1 and lens[s] = keep[s].  When a length does not fit its table row or
+ * become -1 and lens[s] = keep[s].  The codes and scale of a page that keeps
+ * some tokens stay as the dropped ones left them.  When a length does not fit its table row or
  * the stack would grow past free_capacity, nothing changes and
  * IC_DEVFLAG_BAD_ROW is set. */
 typedef struct ic_page_release_args {
@@ -637,7 +638,16 @@ int ic_page_release(const ic_page_release_args* a, void* stream);
  * whatever stood there; later ones keep its scale or, when they need a
  * larger one, raise it and round the page's other codes again to the new unit.
  * Codes are rounded to nearest, ties to even.  Infinities are stored as the
- * largest value, NaN as zero; both set IC_DEVFLAG_NONFINITE.
+ * largest value, NaN as zero; both set IC_DEVFLAG_NONFINITE.  Finite values past
+ * the largest code at 2^60 saturate and set nothing.
+ *
+ * Units only grow while a page is filled, at least twofold each time, so a
+ * value's roundings sum to at most one step of the page's last unit (IC_I8), or
+ * 2^-4 of the value and 2^-9 of the unit (IC_E4M3, whose codes are rounded
+ * again only where they become subnormal), however many tokens raised it.  A
+ * scale never falls again: tokens that are dropped later (rejected drafts,
+ * ic_page_release; a plan that was not committed) leave the kept ones rounded
+ * to the unit that they brought.
  *
  * Two ranges of a write must not share a page, nor must tokens of one range
  * that another page's token or a skipped row stands between: they would race.

@@ -122,7 +122,9 @@ class PagedBatch:
 
     def release(self, keep: Counts) -> None:
         """Session s keeps its first ``keep[s]`` tokens: 0 ends it, a negative
-        number leaves it alone, others drop its newest tokens (rejected drafts)."""
+        number leaves it alone, others drop its newest tokens (rejected drafts).
+        A dropped token that raised its page's scale leaves the page's kept tokens
+        rounded to that scale's unit."""
         page_release(self.lens, self._ints("keep", keep), self.block_table, self.free_pages, self.free_count,
                      status=self.dev_status)
         self.plan = None

@@ -8,7 +8,7 @@ A server that keeps its sessions in 8-bit pages runs, per tick,
   pages back as fp16 / bf16 / fp32;
 * ``paged_attention`` — the new tokens of every session attend over its pages.
 
-``PagedBatch`` (paged_cache) keeps the state of such a server and calls these;
+``PagedBatch`` (paged_batch) keeps the state of such a server and calls these;
 ``process_logits`` (logits) ends the tick.  Caches are ``[H, pool_tokens, D]``
 (one layer) or ``[L, H, pool_tokens, D]`` tensors of ``float8_e4m3fn`` or
 ``int8`` codes with float32 scales ``[..., pool_tokens / 16]``: one power of two
@@ -88,7 +88,8 @@ def page_write(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache:
     may be left out), no row occurs twice, and rows outside the pool are skipped
     (not from among a page's tokens).  A page is written
     in order: tokens that begin at its slot 0 start it anew, later ones keep its
-    scale or raise it (the page's other codes are then rounded again).
+    scale or raise it (the page's other codes are then rounded again; the errors sum
+    to at most one step of the last unit, see the header).
     Infinities are stored as the largest value and NaN as zero; both set
     IC_DEVFLAG_NONFINITE in ``status``.
     """

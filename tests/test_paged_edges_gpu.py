@@ -289,3 +289,48 @@ def test_rows_own_repetition_penalty_rounds_once(dtype):
     f = x.float()
     want = torch.where(f > 0, f / r[:, None], f * r[:, None])
     assert torch.equal(process_logits(x, tokens=said, repetition=r).view(torch.int32), want.view(torch.int32))
+
+
+# ---- a page filled token by token -----------------------------------------------------
+@pytest.mark.parametrize("codes", CODES)
+@pytest.mark.parametrize("growth", [1.0, 1.3, 2.0, 5.0])
+def test_error_of_a_page_filled_token_by_token(codes, growth):
+    """Each token may raise the page's scale and round the older codes once more.
+    Units only grow, by a factor of two or more each time, so the halves of all
+    units that a value was rounded to sum to at most the last unit: |stored - x|
+    <= unit (int8); an e4m3 code that stays normal is not rounded again, and a
+    subnormal one to multiples of 2^-9 of the unit: 2^-4 |x| + 2^-9 unit."""
+    from infercache_b200.paged_ops import page_read, page_write
+    cache = [t[0] for t in empty_cache(1, 3, 2, 64, codes)]
+    x = torch.randn(2, 16, 3, 64, generator=gen(9), device="cuda") * torch.logspace(0, 15, 16, base=growth, device="cuda")[:, None, None]
+    for t in range(16):
+        page_write(x[0, t:t + 1], x[1, t:t + 1], *cache, i32([16 + t]))
+    got = page_read(*cache, i32(list(range(16, 32))), dtype=torch.float32)
+    for g, w, s in zip(got, x, cache[2:]):
+        w, unit = w.transpose(0, 1).double(), s[:, 1].double()[:, None, None]
+        bound = unit if codes == torch.int8 else w.abs() * 2.0 ** -4 + unit * 2.0 ** -9
+        assert bool(((g.double() - w).abs() <= bound).all())
+
+
+@pytest.mark.parametrize("codes", CODES)
+def test_rejected_drafts_leave_the_page_its_unit(codes):
+    """A dropped token that raised its page's scale has rounded the kept ones to the
+    larger unit: within that unit's error, and unchanged by the release."""
+    from infercache_b200 import PagedBatch
+    from test_paged_serving_gpu import make_pool
+    pool = make_pool(codes, L=1, value=torch.float32)
+    b = PagedBatch(pool, 1)
+    x = torch.randn(6, 2, 64, generator=gen(2), device="cuda")
+    x[4:] *= 100
+    b.extend([4])
+    b.append(0, x[:4], x[:4])
+    b.extend([2])
+    b.append(0, x[4:], x[4:])
+    page = int(b.block_table[0, 0])
+    unit = pool.k_scale[0, :, page].clone()
+    before = b.gather(0, 4)[0]
+    b.release([4])
+    assert torch.equal(pool.k_scale[0, :, page], unit) and torch.equal(b.gather(0, 4)[0], before)
+    w = x[:4].transpose(0, 1).double()
+    bound = unit.double()[:, None, None] * (1.0 if codes == torch.int8 else 2.0 ** -9) + (0 if codes == torch.int8 else w.abs() * 2.0 ** -4)
+    assert bool(((before[0].double() - w).abs() <= bound).all())
