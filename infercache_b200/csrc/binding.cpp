@@ -138,6 +138,26 @@ bool rows16(const Tensor& t) {
 }
 bool aligned16(const Tensor& t) { return reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0; }
 
+// Whether the bytes from a tensor's first element to its last meet another's.
+bool meet(const Tensor& a, const Tensor& b) {
+  if (a.numel() == 0 || b.numel() == 0) return false;
+  const auto end = [](const Tensor& t) {
+    int64_t last = 0;
+    for (int64_t i = 0; i < t.dim(); ++i) last += (t.size(i) - 1) * t.stride(i);
+    return reinterpret_cast<uintptr_t>(t.data_ptr()) + (last + 1) * t.element_size();
+  };
+  return reinterpret_cast<uintptr_t>(a.data_ptr()) < end(b) && reinterpret_cast<uintptr_t>(b.data_ptr()) < end(a);
+}
+
+// Whether rows [S, V] of `a` and `b` (contiguous, `stride` bytes apart in both) have
+// none of their bytes in common, though they may alternate.
+bool rows_apart(const Tensor& a, const Tensor& b, int64_t stride) {
+  const auto pa = reinterpret_cast<uintptr_t>(a.data_ptr()), pb = reinterpret_cast<uintptr_t>(b.data_ptr());
+  const Tensor &first = pa <= pb ? a : b, &second = pa <= pb ? b : a;
+  const int64_t shift = static_cast<int64_t>(pa <= pb ? pb - pa : pa - pb) % stride;
+  return shift >= first.size(1) * first.element_size() && shift + second.size(1) * second.element_size() <= stride;
+}
+
 // An uninitialised contiguous tensor on `dev` (made current by the caller).
 Tensor fresh(at::IntArrayRef shape, at::ScalarType type, c10::Device dev) {
   return at::detail::empty_cuda(shape, type, dev, std::nullopt);
@@ -317,6 +337,7 @@ PyObject* py_page_write(PyObject*, PyObject* const* a, Py_ssize_t n) {
                     shape_text(c.k->sizes()) + ", got " + shape_text(k.sizes()) + " and " + shape_text(v.sizes()));
     if (k.scalar_type() != v.scalar_type() || k.device() != c.dev || v.device() != c.dev)
       bad(name, "k and v must share the cache's device and a dtype");
+    if (meet(*c.k, *c.v) || meet(*c.ks, *c.vs)) bad(name, "k_cache and v_cache, and their scales, must not overlap");
     const int dt = float_code(name, k.scalar_type());
     const int64_t N = k.size(d - 3);
     Tensor slots = slots_of(name, a[6], c.dev);
@@ -369,6 +390,7 @@ PyObject* py_page_read(PyObject*, PyObject* const* a, Py_ssize_t n) {
         if (t->sizes() != at::IntArrayRef(shape) || t->scalar_type() != k.scalar_type() || t->device() != c.dev ||
             !t->is_contiguous() || !aligned16(*t))
           bad(name, "out must be two contiguous, 16-byte aligned " + shape_text(shape) + " tensors on " + c.dev.str());
+      if (meet(k, v)) bad(name, "out's tensors must not overlap");
     }
     const int dt = float_code(name, k.scalar_type());
     if (N > 0 && c.L > 0 && c.H > 0) {
@@ -422,6 +444,8 @@ PyObject* py_paged_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
       if (out.sizes() != q.sizes() || out.scalar_type() != type || out.device() != c.dev || !out.is_contiguous() ||
           !aligned16(out))
         bad(name, "out must be a contiguous, 16-byte aligned tensor like q");
+      // a row of q is read by those alone that write the same row of out, before they do
+      if (meet(q, out) && (q.data_ptr() != out.data_ptr() || !q.is_contiguous())) bad(name, "out must be q or not overlap it");
     }
     const bool want_lse = truth(a[11]);
     if (want_lse) lse = fresh({N, Hq}, at::kFloat, c.dev);
@@ -499,6 +523,10 @@ PyObject* py_process_logits(PyObject*, PyObject* const* a, Py_ssize_t n) {
       if (out.scalar_type() != at::kFloat || out.sizes() != x.sizes() || out.device() != dev || out.stride(1) != 1 ||
           (S > 1 && out.stride(0) < V))
         bad(name, "out must be a float32 " + shape_text(x.sizes()) + " tensor with contiguous rows on " + dev.str());
+      const bool alike = S == 1 || out.stride(0) * 4 == x.stride(0) * x.element_size();
+      if (meet(x, out) && !(alike && x.scalar_type() == at::kFloat && x.data_ptr() == out.data_ptr()) &&
+          !(alike && S > 1 && rows_apart(x, out, out.stride(0) * 4)))
+        bad(name, "out must be logits or not overlap them");
     }
     Tensor tok, tl, pl, ids, vals, bl, mask;
     if (!none(a[1])) tok = ints(name, "tokens", tensor(a[1], name, "tokens"), dev, {S, -1});

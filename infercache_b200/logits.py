@@ -37,7 +37,8 @@ def process_logits(logits: torch.Tensor, *, tokens: Optional[torch.Tensor] = Non
     ``logits`` [S, V] is fp32, fp16 or bf16 with contiguous rows; penalties are
     numbers or [S] tensors; missing lengths mean the whole
     row, no prompt.  Ids outside the vocabulary are skipped, so rows may be
-    padded with -1.  ``out`` may be ``logits`` itself when it is float32.
+    padded with -1.  ``out`` may be ``logits`` itself when it is float32, and does
+    not overlap it otherwise.
     """
     return _lib.binding().process_logits(logits, tokens, token_lens, prompt_lens, repetition, presence, frequency,
                                          bias_ids, bias_values, bias_lens, mask, out)

@@ -123,7 +123,7 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     and only steers the choice of kernel.  Returns out [N, Hq, D] in q's dtype,
     with ``return_lse`` also the float32 [N, Hq] natural-log log-sum-exp.  A
     query with nothing to attend over gets zeros and -inf; rows of ``out`` past
-    ``q_start[S]`` are left as they were.  ``out`` may be ``q``.
+    ``q_start[S]`` are left as they were.  ``out`` is ``q`` or does not overlap it.
     """
     return _lib.binding().paged_attention(q, k_cache, v_cache, k_scale, v_scale, block_table, lens, q_start, scale,
                                           max_count, out, return_lse, status)

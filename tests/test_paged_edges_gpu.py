@@ -334,3 +334,38 @@ def test_rejected_drafts_leave_the_page_its_unit(codes):
     w = x[:4].transpose(0, 1).double()
     bound = unit.double()[:, None, None] * (1.0 if codes == torch.int8 else 2.0 ** -9) + (0 if codes == torch.int8 else w.abs() * 2.0 ** -4)
     assert bool(((before[0].double() - w).abs() <= bound).all())
+
+
+# ---- outputs over inputs ---------------------------------------------------------------------
+def test_overlaps_that_would_race_are_refused():
+    from infercache_b200.logits import process_logits
+    from infercache_b200.paged_ops import page_read, page_write, paged_attention
+    k, v, ks, vs = [t[0] for t in empty_cache(1, 2, 3, 64, torch.int8)]
+    rows, slots = torch.randn(2, 2, 64, device="cuda").half(), i32([16, 17])
+    for bad in ((k, k, ks, vs), (k, v, ks, ks)):
+        with pytest.raises(ValueError):
+            page_write(rows, rows, *bad, slots)
+    out = torch.empty(2, 2, 64, device="cuda").half()
+    with pytest.raises(ValueError):
+        page_read(k, v, ks, vs, slots, out=(out, out))
+    x = attention_inputs(1, [40], [3], 2, 2, 64, torch.int8, torch.float16)
+    buf = torch.zeros(4 * 4 * 64 + 64, device="cuda").half()
+    buf[:3 * 256].copy_(x[0].reshape(-1))
+    for q, o in ((buf[:768].view(3, 4, 64), buf[64:832].view(3, 4, 64)),
+                 (buf[:960].as_strided((3, 4, 64), (320, 64, 1)), buf[:768].view(3, 4, 64))):
+        with pytest.raises(ValueError):
+            paged_attention(q, *x[1:], out=o)
+    wide = torch.randn(5, 300, device="cuda")[:4]
+    for a, o in ((wide[:, :100], wide[:, 50:150]), (wide[:, :100], wide[:, 250:300].as_strided((4, 100), (300, 1))),
+                 (wide[:, :100], wide.view(-1)[:400].view(4, 100)), (wide[:3], wide[1:4]),
+                 (wide.view(torch.float16)[:, :100], wide[:, :100])):
+        with pytest.raises(ValueError):
+            process_logits(a, out=o)
+    tok = i32([[1, 2], [3, 4], [5, 6], [7, 99]])
+    want = process_logits(wide[:, :100].clone(), tokens=tok, repetition=1.5)
+    got = process_logits(wide[:, :100], tokens=tok, repetition=1.5, out=wide[:, 100:200])  # side by side
+    assert torch.equal(got, want)
+    got = process_logits(wide[:, 200:], tokens=tok, repetition=1.5, out=wide[:, :100])
+    assert torch.equal(got, process_logits(wide[:, 200:].clone(), tokens=tok, repetition=1.5))
+    got = process_logits(wide[:1, :100], out=wide[:1, 100:200])
+    assert torch.equal(got, wide[:1, :100])
