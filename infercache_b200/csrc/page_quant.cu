@@ -1,16 +1,17 @@
 // Rows into and out of 8-bit pages.
 //
 // Write: one warp per (page run, layer and head, K or V) -- a run is the
-// tokens of one call that land in one page, one after another.  The run's rows pass through a few
-// vectors per lane: their largest magnitude gives the page scale's exponent, then
-// the codes are stored; a run that does not start its page and needs a larger
+// tokens of one call in consecutive slots of one page.  The run's rows pass through
+// a few vectors per lane: their largest magnitude gives the page scale's exponent,
+// then the codes are stored; a run that does not start its page and needs a larger
 // scale first rounds the page's other codes again.  Read: one thread per
 // 8 codes of RT tokens.  Both are bound by HBM (a write moves size + 1 bytes per
 // element, a read 1 + size) as long as an element costs few instructions, which
 // is why maxima and fp16 codes are taken two at a time.  Measured (B200): 16
 // prompts of 2048 fp16 tokens, 36 layers, 2 heads, 128 dims, written as int8 and
-// read back: 600 to 632 us for 3.62 GB, 88 to 92 % of a plain copy's rate; one token
-// of 64 sessions, 4 heads, written and read back: 8.9 us, the calls' host time.
+// read back: 600 to 636 us for 3.62 GB, 87 to 92 % of a plain copy's rate (the read
+// alone 339); one token of 64 sessions, 4 heads, written and read back: 8 to 9 us, the
+// calls' host time.
 #include <stdio.h>
 
 #include <type_traits>

@@ -15,10 +15,11 @@
 // Nothing depends on an order of atomics.
 //
 // Measured (B200, 128 dims): 64 sessions of 1k to 8k tokens, 4 KV heads of 7 query
-// heads, 57 us: 5.2 TB/s of codes and scales, 80 % of a plain copy's rate; 16
-// of 2k, 2 heads of 8, 12.2 us (clusters of 8); one of 128k, as many heads, 23.8 us,
-// of which the join is 4; one of 300 tokens 6.8 us (launch and
-// dependent loads: q, table, scales, pages).
+// heads, 57 to 60 us: 5.2 TB/s of codes and scales, 78 to 80 % of a plain copy's
+// rate; 16 of 2k, 2 heads of 8, 12.2 us (clusters of 8; 15.4 under a table of 2048
+// columns); one of 128k, as many heads, 23.8 us, of which the join is 4; one of 300
+// tokens 6.7 us (launch and dependent loads: q, table, scales, pages; 9.3 under
+// 2048 columns).
 //
 // Inside a CTA each warp streams its own pages (every 8th of the segment)
 // through a ring of its own: one elected lane issues two TMA box copies per
