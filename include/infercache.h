@@ -690,7 +690,8 @@ int ic_page_read_q8(const ic_page_q8_args* a, void* stream);
  * IC_DEVFLAG_BAD_ROW and their tokens are left out.  Rows of a page behind the
  * session's last token are never used, whatever they hold.
  * Products are exact and summed in 32 bits; softmax weights enter the second
- * product as fp16 (relative error 2^-11), bf16 queries the first as fp16 after a
+ * product as fp16 (relative error 2^-11, or 2^-32 of the row's largest product
+ * of a weight and its page's V scale), bf16 queries the first as fp16 after a
  * power of two per row (exact down to 2^-27 of the row's largest element).
  * k, v: one layer's codes [Hkv, pool_tokens, D] and scales [Hkv, pool_tokens /
  * 16]; q has strides (elements), out is [num_q_tokens, Hq, D] contiguous in
